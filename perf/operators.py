@@ -38,11 +38,11 @@ def listed():
         # the norm of a training step, with the gradient that arrives at the sum
         dict(name="norm_train", op="norm", rows=16384, C=4096, dtype="bf16", residual=True, fp8=False, train=True),
         # the projection of one frame of each of 4 streams: the weights are read once
-        dict(name="gemm_token", op="gemm", M=4, N=8192, K=4096, out="bf16", quantize=False),
+        dict(name="gemm_token", op="gemm", M=4, N=8192, K=4096, quantize=False),
         # the projection behind a scan: activations are put in 8 bits within the call; an odd number of rows
-        dict(name="gemm_frames", op="gemm", M=777, N=2056, K=4096, out="bf16", quantize=True),
+        dict(name="gemm_frames", op="gemm", M=777, N=2056, K=4096, quantize=True),
         # the projection of a long batch
-        dict(name="gemm_prompt", op="gemm", M=8192, N=8192, K=4096, out="bf16", quantize=False),
+        dict(name="gemm_prompt", op="gemm", M=8192, N=8192, K=4096, quantize=False),
     ]
 
 
@@ -70,8 +70,7 @@ def draw(rng):
             ok = c["rows"] * c["C"] <= 1 << 26
         else:
             c = dict(op=op, M=_spread(rng, 1, 8192), N=_spread(rng, 16, 16384), K=16 * _spread(rng, 4, 1024),
-                     out=rng.choice(("bf16", "bf16", "f32")), quantize=False)
-            c["quantize"] = c["out"] == "bf16" and rng.random() < 0.5
+                     quantize=rng.random() < 0.5)
             ok = c["M"] * c["N"] * c["K"] <= 1 << 37
         if ok:
             return c
@@ -190,7 +189,7 @@ def _plain_gemm(s):
     a8, sa = _quantize_rows(s["a"].float()) if case["quantize"] else (s["a8"], s["a_scales"])
     a = a8.float() * sa.repeat_interleave(128, 1)[:, :case["K"]]
     b = s["b8"].float() * s["b_scales"].repeat_interleave(128, 0)[:case["N"]].repeat_interleave(128, 1)[:, :case["K"]]
-    return {"out": (a @ b.t()).to(_dtype(case["out"]))}
+    return {"out": (a @ b.t()).to(torch.bfloat16)}
 
 
 def _plain_norm(s):
@@ -313,7 +312,7 @@ def _own_gemm(s):
         ops.quantize_fp8(s["a"], a8, sa)
     else:
         a8, sa = s["a8"], s["a_scales"]
-    out = torch.empty(M, N, dtype=_dtype(case["out"]), device="cuda")
+    out = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
     ops.gemm_nt_fp8(a8, sa, s["b8"], s["b_scales"], out)
     return {"out": out}
 
@@ -426,7 +425,7 @@ def work(case):
     M, N, K = case["M"], case["N"], case["K"]
     kb = -(-K // 128)
     size = M * K * (2 if case["quantize"] else 1) + (0 if case["quantize"] else 4 * M * kb) + N * K + 4 * -(-N // 128) * kb
-    return {"bytes": size + M * N * (2 if case["out"] == "bf16" else 4), "flops": 2 * M * N * K}
+    return {"bytes": size + M * N * 2, "flops": 2 * M * N * K}
 
 
 # ------------------------------------------------------------------------------------------------- 64-bit values

@@ -36,6 +36,10 @@ extern "C" {
 #define SLAMHIP_E_HIP (-2)      /* a HIP runtime call or kernel launch failed */
 #define SLAMHIP_E_SIZE (-3)     /* size beyond what the entry point supports */
 
+/* element types of the sequence-layer entry points */
+#define SLAMHIP_F32 0
+#define SLAMHIP_BF16 1
+
 /* number of reduced quantities per (pair, neighbour) */
 #define SLAMHIP_NSUMS 4         /* sum|r_photo|, sum r_photo^2, sum|r_geo|, sum r_geo^2 */
 #define SLAMHIP_NCOUNTS 4       /* n_valid0, n_inb, n_warp, n_geo */
@@ -494,6 +498,80 @@ int slamhip_lrn_bwd_add(const void* x, const void* dy, void* dx, long long P, in
 /* float32 [P][C] -> bfloat16 [P][Cp] with zero channels C..Cp-1 (the 3- or 4-channel
  * network input widened to the 8 channels im2col works in). */
 int slamhip_pad_cast_bf16(const float* src, void* dst, long long P, int C, int Cp, void* stream);
+
+/* ---- device: sequence layers --------------------------------------------------
+ * Operators over sequences of frames, beside the recurrent head (slam/network/lstm_model.py:25-49 is the reference's only
+ * sequence model).  `dtype` (SLAMHIP_F32 / SLAMHIP_BF16) is the type of the activations and of their gradients; parameters,
+ * their gradients, statistics and recurrent states are float32.  Elements need their own alignment alone.  Outputs are fully
+ * overwritten and overlap no input except where said.  Sums have a fixed order: identical inputs give identical bits.
+ *
+ * Root-mean-square norm of the rows of x [rows][C] (C <= 16384): s = x + residual, rounded to `dtype` (sum_out; residual and
+ * sum_out may be NULL: s = x), rstd = (mean(s^2) + eps)^(-1/2), y = s rstd weight.  Outputs, each may be NULL but one:
+ * sum_out, y, and y8 uint8 [rows][C] (e4m3) with scales float32 [rows][ceil(C/128)]: scale = max(max|y| / 448, 2^-100) over
+ * 128 consecutive values of the unrounded y, y8 = the nearest of y / scale.  rstd float32 [rows] (may be NULL) is kept for the
+ * backward pass.  y or sum_out may be x or residual itself. */
+int slamhip_rms_norm_fwd(const void* x, const void* residual, const float* weight, float eps, long long rows, int C, int dtype,
+                         void* sum_out, void* y, void* y8, float* scales, float* rstd, void* stream);
+/* dx = the gradient at x and at residual: rstd (w dy - hat mean(w dy hat)) + d_sum with hat = s rstd; `sum` is s (sum_out, or x
+ * without a residual), d_sum the gradient that arrives at sum_out (may be NULL).  dweight [C].  dx may be dy, or d_sum. */
+size_t slamhip_rms_norm_bwd_workspace_bytes(long long rows, int C);
+int slamhip_rms_norm_bwd(const void* dy, const void* sum, const float* weight, const float* rstd, const void* d_sum, long long rows,
+                         int C, int dtype, void* dx, float* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* x [rows][C] -> q uint8 [rows][C] (e4m3) and a scale for each 128 consecutive values of a row, scales [rows][ceil(C/128)]: the
+ * rule of slamhip_rms_norm_fwd.  A NaN makes its whole block NaN, an infinity makes its block's scale infinite. */
+int slamhip_quantize_fp8(const void* x, long long rows, int C, int dtype, void* q, float* scales, void* stream);
+/* The same with a scale for each 128 x 128 block: scales [ceil(R/128)][ceil(C/128)] (weights, laid out once). */
+int slamhip_quantize_fp8_blocks(const void* x, int R, int C, int dtype, void* q, float* scales, void* stream);
+
+/* out [M][N] bfloat16 = sum over blocks kb of 128 of a_scales[m][kb] b_scales[n/128][kb] sum_k a[m][k]
+ * b[n][k], for a uint8 [M][K] and b uint8 [N][K] in e4m3 with a_scales float32 [M][ceil(K/128)] and b_scales float32
+ * [ceil(N/128)][ceil(K/128)].  K a multiple of 16, a and b 16-byte aligned and below 4 GB each; M and N are free.
+ * Block sums are float32 except inside the matrix unit, which adds eight products at a time after cutting each to 2^-13 of the
+ * largest one's power of two. */
+int slamhip_gemm_nt_fp8(const void* a, const float* a_scales, const void* b, const float* b_scales, int M, int N, int K, void* out,
+                        void* stream);
+
+/* Sequences are [B][T][C] with unit stride over C and any stride, in elements, of a sequence and of a step: `strides` (host
+ * memory) holds {sequence, step} of each in the order named.  lengths int32 [B] (NULL: all T; values are clamped to 0..T): rows
+ * at and behind a sequence's length are never used, whatever they hold, and are zero in y and in the gradients.
+ *
+ * Short causal convolution over time with a filter for each channel, weight [C][K], 2 <= K <= 4: pre = bias + sum_k w[c][k]
+ * xp[t + k], y = pre (silu == 0) or pre / (1 + e^-pre), where xp is the K - 1 rows of state_in [B][K-1][C] (NULL: zeros) and
+ * then x.  state_out [B][K-1][C] (NULL, or state_in itself): the last K - 1 rows of xp up to the sequence's length, which
+ * continue it in a later call; one frame at a time is T = 1.  strides: x, y.  bias may be NULL. */
+int slamhip_causal_conv_fwd(const void* x, const long long* strides, const float* weight, const float* bias, const void* state_in,
+                            const int32_t* lengths, int B, int T, int C, int K, int silu, int dtype, void* y, void* state_out,
+                            void* stream);
+/* dx, dweight [C][K], dbias [C] (may be NULL) and d_state_in [B][K-1][C] (may be NULL) from dy and from d_state_out, the
+ * gradient that arrives at state_out (may be NULL).  strides: dy, x, dx. */
+size_t slamhip_causal_conv_bwd_workspace_bytes(int B, int T, int C, int K);
+int slamhip_causal_conv_bwd(const void* dy, const void* x, const long long* strides, const float* weight, const float* bias,
+                            const void* state_in, const void* d_state_out, const int32_t* lengths, int B, int T, int C, int K, int silu,
+                            int dtype, void* dx, float* dweight, float* dbias, void* d_state_in, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Selective scan over sequences u, delta, z, y [B][T][C] and Bm, Cm [B][T][N], N <= 32: dt = softplus(delta + delta_bias) (delta +
+ * delta_bias itself with softplus == 0), h_t[c][n] = exp(dt A[c][n]) h_{t-1}[c][n] + dt u Bm[n], y = (sum_n Cm[n] h_t[c][n] +
+ * D[c] u) z / (1 + e^-z).  D, delta_bias, z may be NULL (no such term; no gate).  state_in [B][C][N] (NULL: zeros) is h before
+ * the first step, state_out [B][C][N] (NULL, or state_in itself) h after the sequence's last step; one frame at a time is T = 1.
+ * kept_states: slamhip_selective_scan_kept_floats floats for the backward pass, or NULL.
+ * strides: u, delta, z, Bm, Cm, y (z's may be anything without z). */
+size_t slamhip_selective_scan_kept_floats(int B, int T, int C, int N);
+size_t slamhip_selective_scan_fwd_workspace_bytes(int B, int T, int C, int N);
+int slamhip_selective_scan_fwd(const void* u, const void* delta, const void* z, const void* Bm, const void* Cm, const long long* strides,
+                               const float* A, const float* D, const float* delta_bias, const float* state_in, const int32_t* lengths,
+                               int B, int T, int C, int N, int softplus, int dtype, void* y, float* state_out, float* kept_states,
+                               void* workspace, size_t workspace_bytes, void* stream);
+/* All gradients from dy and d_state_out (the gradient that arrives at state_out, may be NULL): du, ddelta, dz (with z) like u,
+ * dB, dC [B][T][N], dA [C][N], dD, d_delta_bias [C] (may be NULL), d_state_in [B][C][N] (may be NULL).  kept_states are the
+ * forward pass's of the same inputs.  strides: dy, u, delta, z, Bm, Cm, du, ddelta, dz, dB, dC. */
+size_t slamhip_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N);
+int slamhip_selective_scan_bwd(const void* dy, const void* u, const void* delta, const void* z, const void* Bm, const void* Cm,
+                               const long long* strides, const float* A, const float* D, const float* delta_bias,
+                               const float* kept_states, const float* d_state_out, const int32_t* lengths, int B, int T, int C, int N,
+                               int softplus, int dtype, void* du, void* ddelta, void* dz, void* dB, void* dC, float* dA, float* dD,
+                               float* d_delta_bias, float* d_state_in, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -108,6 +108,20 @@ SIGNATURES = {
     "slamhip_lrn_fwd": ([_c_void_p] * 2 + [ctypes.c_longlong, _c_int, _c_int] + [ctypes.c_float] * 3 + [_c_void_p], _c_int),
     "slamhip_lrn_bwd_add": ([_c_void_p] * 3 + [ctypes.c_longlong, _c_int, _c_int] + [ctypes.c_float] * 3 + [_c_void_p], _c_int),
     "slamhip_pad_cast_bf16": ([_c_void_p] * 2 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p], _c_int),
+    "slamhip_rms_norm_fwd": ([_c_void_p] * 3 + [ctypes.c_float, ctypes.c_longlong, _c_int, _c_int] + [_c_void_p] * 6, _c_int),
+    "slamhip_rms_norm_bwd_workspace_bytes": ([ctypes.c_longlong, _c_int], ctypes.c_size_t),
+    "slamhip_rms_norm_bwd": ([_c_void_p] * 5 + [ctypes.c_longlong, _c_int, _c_int] + [_c_void_p] * 3 + [ctypes.c_size_t, _c_void_p], _c_int),
+    "slamhip_quantize_fp8": ([_c_void_p, ctypes.c_longlong, _c_int, _c_int] + [_c_void_p] * 3, _c_int),
+    "slamhip_quantize_fp8_blocks": ([_c_void_p, _c_int, _c_int, _c_int] + [_c_void_p] * 3, _c_int),
+    "slamhip_gemm_nt_fp8": ([_c_void_p] * 4 + [_c_int] * 3 + [_c_void_p] * 2, _c_int),
+    "slamhip_causal_conv_fwd": ([_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p] * 3, _c_int),
+    "slamhip_causal_conv_bwd_workspace_bytes": ([_c_int] * 4, ctypes.c_size_t),
+    "slamhip_causal_conv_bwd": ([_c_void_p] * 8 + [_c_int] * 6 + [_c_void_p] * 5 + [ctypes.c_size_t, _c_void_p], _c_int),
+    "slamhip_selective_scan_kept_floats": ([_c_int] * 4, ctypes.c_size_t),
+    "slamhip_selective_scan_fwd_workspace_bytes": ([_c_int] * 4, ctypes.c_size_t),
+    "slamhip_selective_scan_fwd": ([_c_void_p] * 11 + [_c_int] * 6 + [_c_void_p] * 4 + [ctypes.c_size_t, _c_void_p], _c_int),
+    "slamhip_selective_scan_bwd_workspace_bytes": ([_c_int] * 4, ctypes.c_size_t),
+    "slamhip_selective_scan_bwd": ([_c_void_p] * 13 + [_c_int] * 6 + [_c_void_p] * 10 + [ctypes.c_size_t, _c_void_p], _c_int),
     "slamhip_adam_step": ([_c_void_p] * 4 + [ctypes.c_longlong] + [ctypes.c_float] * 4 + [_c_int, ctypes.c_float,
                                                                                           _c_void_p], _c_int),
     "slamhip_adam_step_dev": ([_c_void_p] * 4 + [ctypes.c_longlong, _c_void_p] + [ctypes.c_float] * 4 +

@@ -1,0 +1,331 @@
+// Short causal convolution over time, one filter a channel, with an optional SiLU, and its backward pass.
+//
+//   pre[b,t,c] = bias[c] + sum_k w[c,k] xp[b,t+k,c],  y = pre sigmoid(pre)      xp = K - 1 rows of state, then x
+//   backward: d = dy silu'(pre),  dxp[p] = sum_k w[k] d[p-k],  dw[c,k] = sum d[t] xp[t+k],  dbias = sum d
+//
+// A thread walks one octet of channels down a run of time steps with the last K rows in registers, so a row is read from memory
+// once but for the K - 1 rows in front of a run (and, backward, as many behind it).  Nothing but the bytes bounds this.
+#include <hip/hip_runtime.h>
+
+#include "common.h"
+#include "sequence_device.h"
+
+namespace slamhip {
+namespace {
+
+struct ConvArgs {
+  const void *x, *dy, *state_in, *d_state_out;
+  const float *w, *bias;
+  void *y, *state_out, *dx, *d_state_in;
+  float* part;
+  const int* lengths;
+  long long xb, xt, yb, yt, dyb, dyt, dxb, dxt;   // strides of a sequence and of a time step, in elements
+  int T, C, run, runs, silu;
+  int lx_log2;   // a workgroup is 2^lx_log2 octets by 256 / 2^lx_log2 runs
+};
+
+struct Place {
+  int c, n, run, t0;
+};
+
+__device__ __forceinline__ Place conv_place(const ConvArgs& a) {
+  const int lx = 1 << a.lx_log2;
+  Place p;
+  p.c = (blockIdx.x * lx + (threadIdx.x & (lx - 1))) * 8;
+  p.n = a.C - p.c;
+  p.run = blockIdx.y * (256 >> a.lx_log2) + (threadIdx.x >> a.lx_log2);
+  p.t0 = p.run * a.run;
+  return p;
+}
+
+__device__ __forceinline__ int conv_length(const ConvArgs& a, int b) {
+  if (!a.lengths) return a.T;
+  const int n = a.lengths[b];
+  return n < 0 ? 0 : (n > a.T ? a.T : n);
+}
+
+// row `t` of a sequence: state rows in front of it, zeros where it has neither
+template <typename T, int K>
+__device__ __forceinline__ f32x8 conv_row(const ConvArgs& a, const T* x, const T* state, int t, int len, int c, int n) {
+  if (t >= 0) return t < len ? load8(x + t * a.xt + c, n) : f32x8{};
+  return state ? load8(state + (long long)(t + K - 1) * a.C + c, n) : f32x8{};
+}
+
+template <int K>
+__device__ __forceinline__ void conv_weights(const ConvArgs& a, int c, int n, f32x8 (&w)[K], f32x8& bias) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    bias[j] = a.bias && j < n ? a.bias[c + j] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][j] = j < n ? a.w[(long long)(c + j) * K + k] : 0.0f;
+  }
+}
+
+template <typename T, int K>
+__global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
+  const Place p = conv_place(a);
+  const int b = blockIdx.z, len = conv_length(a, b);
+  if (p.n <= 0 || p.run >= a.runs) return;
+  const T* x = (const T*)a.x + b * a.xb;
+  T* y = (T*)a.y + b * a.yb;
+  const T* state = a.state_in ? (const T*)a.state_in + (long long)b * (K - 1) * a.C : nullptr;
+  f32x8 w[K], bias, win[K];
+  conv_weights<K>(a, p.c, p.n, w, bias);
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) win[k] = conv_row<T, K>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
+  if (p.run == 0 && a.state_out) {   // win holds the state: it may be written over from here on
+    T* out = (T*)a.state_out + (long long)b * (K - 1) * a.C;
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) {
+      f32x8 v{};
+      if (len + i >= K - 1) v = load8(x + (len + i - (K - 1)) * a.xt + p.c, p.n);
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+        if (len + i == k) v = win[k];
+      store8(out + (long long)i * a.C + p.c, v, p.n);
+    }
+  }
+  const int t1 = min(p.t0 + a.run, a.T);
+  for (int t = p.t0; t < t1; t += 4) {
+    f32x8 next[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next[i] = t + i < t1 ? conv_row<T, K>(a, x, nullptr, t + i, len, p.c, p.n) : f32x8{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      win[K - 1] = next[i];
+      f32x8 v = bias;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = fmaf(w[k][j], win[k][j], v[j]);
+      if (a.silu)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= sigmoid_(v[j]);
+      if (t + i >= len) v = f32x8{};
+      if (t + i < t1) store8(y + (t + i) * a.yt + p.c, v, p.n);
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) win[k] = win[k + 1];
+    }
+  }
+}
+
+// part [sequence][group of runs][K + 1][C]: dw and dbias of a workgroup's runs
+template <typename T, int K>
+__global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
+  __shared__ float sh[256 * 8];
+  const Place p = conv_place(a);
+  const int b = blockIdx.z, len = conv_length(a, b);
+  const bool live = p.n > 0 && p.run < a.runs;
+  f32x8 dw[K], db{};
+#pragma unroll
+  for (int k = 0; k < K; ++k) dw[k] = f32x8{};
+  if (live) {
+    const T* x = (const T*)a.x + b * a.xb;
+    const T* dy = (const T*)a.dy + b * a.dyb;
+    T* dx = (T*)a.dx + b * a.dxb;
+    const long long sbase = (long long)b * (K - 1) * a.C;
+    const T* state = a.state_in ? (const T*)a.state_in + sbase : nullptr;
+    const T* d_out = a.d_state_out ? (const T*)a.d_state_out + sbase : nullptr;
+    T* d_in = a.d_state_in ? (T*)a.d_state_in + sbase : nullptr;
+    f32x8 w[K], bias, win[K], d[K];
+    conv_weights<K>(a, p.c, p.n, w, bias);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      d[k] = f32x8{};   // d[k] is the gradient at pre of step t - (K - 1) + k
+      if (k < K - 1) win[k] = conv_row<T, K>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
+    }
+    const int t1 = min(p.t0 + a.run, a.T);
+    const int first = p.run == 0 ? -(K - 1) : p.t0;   // the first run's rows begin with the state's
+    for (int t = p.t0; t < t1 + K - 1; t += 2) {
+      f32x8 nx[2], ny[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool in = t + i < t1 + K - 1 && t + i < len;
+        nx[i] = in ? load8(x + (t + i) * a.xt + p.c, p.n) : f32x8{};
+        ny[i] = in ? load8(dy + (t + i) * a.dyt + p.c, p.n) : f32x8{};
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int now = t + i;
+        if (now < t1 + K - 1) {
+          win[K - 1] = nx[i];
+          f32x8 g{};
+          if (now < len) {
+            g = ny[i];
+            if (a.silu) {
+              f32x8 pre = bias;
+#pragma unroll
+              for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pre[j] = fmaf(w[k][j], win[k][j], pre[j]);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float s = sigmoid_(pre[j]);
+                g[j] *= s * fmaf(pre[j], 1.0f - s, 1.0f);
+              }
+            }
+          }
+          d[K - 1] = g;
+          if (now < t1) {
+            db += g;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) dw[k][j] = fmaf(g[j], win[k][j], dw[k][j]);
+          }
+          const int row = now - (K - 1);
+          if (row >= first) {
+            f32x8 v{};
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = fmaf(w[k][j], d[K - 1 - k][j], v[j]);
+            const int i_state = row - len + K - 1;   // row of the state that leaves
+            if (d_out && i_state >= 0 && i_state < K - 1) v += load8(d_out + (long long)i_state * a.C + p.c, p.n);
+            if (row >= 0) {
+              if (row >= len) v = f32x8{};
+              store8(dx + row * a.dxt + p.c, v, p.n);
+            } else if (d_in) {
+              store8(d_in + (long long)(row + K - 1) * a.C + p.c, v, p.n);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < K - 1; ++k) {
+            win[k] = win[k + 1];
+            d[k] = d[k + 1];
+          }
+        }
+      }
+    }
+  }
+  // the workgroup's runs meet in shared memory, in order
+  const int lx = 1 << a.lx_log2, ly = 256 >> a.lx_log2;
+  float* part = a.part + ((long long)b * gridDim.y + blockIdx.y) * (K + 1) * a.C;
+#pragma unroll
+  for (int k = 0; k <= K; ++k) {
+    const f32x8 v = k < K ? dw[k < K ? k : 0] : db;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sh[j * 256 + threadIdx.x] = v[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < lx * 8; i += 256) {   // i = channel within the workgroup's
+      float s = 0.0f;
+      for (int r = 0; r < ly; ++r) s += sh[(i & 7) * 256 + r * lx + (i >> 3)];
+      const int c = blockIdx.x * lx * 8 + i;
+      if (c < a.C) part[(long long)k * a.C + c] = s;
+    }
+  }
+}
+
+struct ConvShape {
+  int run, runs, lx_log2, gx, gy;
+};
+
+// Runs are as long as leaves about eight waves a SIMD (fewer rows are read twice); short sequences take shorter ones.
+ConvShape conv_shape(int B, int T, int C, int longest, int align) {
+  ConvShape s;
+  const int octets = (C + 7) / 8;
+  s.lx_log2 = 0;
+  while (s.lx_log2 < 6 && (1 << s.lx_log2) < octets) ++s.lx_log2;
+  s.gx = (octets + (1 << s.lx_log2) - 1) >> s.lx_log2;
+  const long long rows_per_thread = (long long)B * T * octets / (8192LL * 64);
+  long long run = (rows_per_thread + align - 1) / align * align;
+  if (run < align) run = align;
+  if (run > longest) run = longest;
+  s.run = (int)run;
+  s.runs = T > 0 ? (T + s.run - 1) / s.run : 1;
+  const int ly = 256 >> s.lx_log2;
+  s.gy = (s.runs + ly - 1) / ly;
+  return s;
+}
+
+constexpr int kFwdLongest = 16, kFwdAlign = 4, kBwdLongest = 64, kBwdAlign = 8;
+
+template <typename T>
+int conv_fwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {
+  if (K == 2) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 2>), grid, dim3(256), 0, s, a);
+  if (K == 3) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 3>), grid, dim3(256), 0, s, a);
+  if (K == 4) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 4>), grid, dim3(256), 0, s, a);
+  SLAMHIP_HIP(hipGetLastError());
+  return SLAMHIP_OK;
+}
+
+template <typename T>
+int conv_bwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {
+  if (K == 2) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 2>), grid, dim3(256), 0, s, a);
+  if (K == 3) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 3>), grid, dim3(256), 0, s, a);
+  if (K == 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 4>), grid, dim3(256), 0, s, a);
+  SLAMHIP_HIP(hipGetLastError());
+  return SLAMHIP_OK;
+}
+
+// part's columns are [K + 1][C]; dweight is [C][K]
+struct ConvGradients {
+  float *dw, *db;
+  int C, K;
+  __device__ void operator()(int i, float v) const {
+    const int k = i / C, c = i - k * C;
+    if (k < K)
+      dw[(long long)c * K + k] = v;
+    else if (db)
+      db[c] = v;
+  }
+};
+
+}  // namespace
+}  // namespace slamhip
+
+using namespace slamhip;
+
+extern "C" {
+
+int slamhip_causal_conv_fwd(const void* x, const long long* strides, const float* weight, const float* bias, const void* state_in,
+                            const int32_t* lengths, int B, int T, int C, int K, int silu, int dtype, void* y, void* state_out,
+                            void* stream) {
+  SLAMHIP_REQUIRE(B >= 0 && T >= 0 && C > 0 && K >= 2 && K <= 4 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG,
+                  "causal_conv_fwd: need C >= 1, 2 <= K <= 4 and a known type");
+  SLAMHIP_REQUIRE(B <= 65535 && T <= (1 << 20) && C <= (1 << 20), SLAMHIP_E_SIZE, "causal_conv_fwd: at most 65535 sequences, 2^20 steps and channels");
+  if (B == 0 || (T == 0 && !state_out)) return SLAMHIP_OK;
+  SLAMHIP_REQUIRE(weight && (T == 0 || (x && y && strides)), SLAMHIP_E_ARG, "causal_conv_fwd: null pointer");
+  ConvArgs a{};
+  a.x = x, a.w = weight, a.bias = bias, a.state_in = state_in, a.y = y, a.state_out = state_out, a.lengths = lengths;
+  if (strides) a.xb = strides[0], a.xt = strides[1], a.yb = strides[2], a.yt = strides[3];
+  const ConvShape g = conv_shape(B, T, C, kFwdLongest, kFwdAlign);
+  a.T = T, a.C = C, a.run = g.run, a.runs = g.runs, a.silu = silu, a.lx_log2 = g.lx_log2;
+  const dim3 grid(g.gx, g.gy, B);
+  SLAMHIP_REQUIRE(g.gy <= 65535, SLAMHIP_E_SIZE, "causal_conv_fwd: too many steps");
+  return dtype == SLAMHIP_BF16 ? conv_fwd<__bf16>(a, K, grid, (hipStream_t)stream) : conv_fwd<float>(a, K, grid, (hipStream_t)stream);
+}
+
+size_t slamhip_causal_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
+  if (B <= 0 || C <= 0 || T < 0 || K < 2) return 0;
+  return (size_t)B * conv_shape(B, T, C, kBwdLongest, kBwdAlign).gy * (K + 1) * C * sizeof(float);
+}
+
+int slamhip_causal_conv_bwd(const void* dy, const void* x, const long long* strides, const float* weight, const float* bias,
+                            const void* state_in, const void* d_state_out, const int32_t* lengths, int B, int T, int C, int K, int silu,
+                            int dtype, void* dx, float* dweight, float* dbias, void* d_state_in, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  SLAMHIP_REQUIRE(B >= 0 && T >= 0 && C > 0 && K >= 2 && K <= 4 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG,
+                  "causal_conv_bwd: need C >= 1, 2 <= K <= 4 and a known type");
+  SLAMHIP_REQUIRE(B <= 65535 && T <= (1 << 20) && C <= (1 << 20), SLAMHIP_E_SIZE, "causal_conv_bwd: at most 65535 sequences, 2^20 steps and channels");
+  SLAMHIP_REQUIRE(weight && dweight && (B == 0 || workspace) && (B == 0 || T == 0 || (dy && x && dx && strides)), SLAMHIP_E_ARG,
+                  "causal_conv_bwd: null pointer");
+  SLAMHIP_REQUIRE(workspace_bytes >= slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K), SLAMHIP_E_ARG, "causal_conv_bwd: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  const ConvShape g = conv_shape(B, T, C, kBwdLongest, kBwdAlign);
+  if (B > 0) {
+    ConvArgs a{};
+    a.x = x, a.dy = dy, a.w = weight, a.bias = bias, a.state_in = state_in, a.d_state_out = d_state_out, a.lengths = lengths;
+    a.dx = dx, a.d_state_in = d_state_in, a.part = (float*)workspace;
+    if (strides) a.dyb = strides[0], a.dyt = strides[1], a.xb = strides[2], a.xt = strides[3], a.dxb = strides[4], a.dxt = strides[5];
+    a.T = T, a.C = C, a.run = g.run, a.runs = g.runs, a.silu = silu, a.lx_log2 = g.lx_log2;
+    SLAMHIP_REQUIRE(g.gy <= 65535, SLAMHIP_E_SIZE, "causal_conv_bwd: too many steps");
+    const int rc = dtype == SLAMHIP_BF16 ? conv_bwd<__bf16>(a, K, dim3(g.gx, g.gy, B), s) : conv_bwd<float>(a, K, dim3(g.gx, g.gy, B), s);
+    if (rc != SLAMHIP_OK) return rc;
+  }
+  SLAMHIP_HIP(column_sums((const float*)workspace, (long long)B * g.gy, (K + 1) * C, ConvGradients{dweight, dbias, C, K}, s));
+  return SLAMHIP_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,667 @@
+// Selective scan: a diagonal linear recurrence for each channel whose step, input and output weights depend on the time step.
+//
+//   dt = softplus(delta + delta_bias);  h_t[n] = exp(dt_t A[n]) h_{t-1}[n] + dt_t u_t B_t[n]
+//   y_t = (sum_n C_t[n] h_t[n] + D u_t) silu(z_t)
+// Backward, with e_t = dy_t silu(z_t) and g_t[n] = e_t C_t[n] + exp(dt_{t+1} A[n]) g_{t+1}[n], q_t = exp(dt_t A) g_t h_{t-1}:
+//   dB_t[n] = sum_c g_t dt_t u_t      dC_t[n] = sum_c e_t h_t       dA[n] = sum_{b,t} q_t dt_t
+//   du_t = dt_t sum_n g_t B_t + D e_t      ddt_t = u_t sum_n g_t B_t + sum_n q_t A      dz_t = dy_t inner_t silu'(z_t)
+//
+// Layout.  Four lanes (a DPP quad) hold one channel, P = N / 4 states each: sums over the states are two quad permutes, a wave
+// is 16 channels.  What is needed once a step and channel (softplus, gates, stores) is done by lane k of the quad for
+// steps k, k + 4, ... and handed on with quad permutes.  B_t and C_t are staged in shared memory in float32 for the workgroup's
+// 64 channels.  Nearly all time goes to vector instructions: an exponential, two products and two multiply-adds for every
+// (step, channel, state).
+// A long sequence is cut into chunks where there are too few channels to fill the chip: a first pass leaves each chunk's own end
+// state and its sum of dt (the decay over a chunk is exp(A sum dt)), and every chunk of the second pass joins those in front of
+// it.  The backward pass runs over the chunks the same way from behind, and recomputes the states of TB steps from the one that
+// the forward pass kept in front of them.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "common.h"
+#include "sequence_device.h"
+
+namespace slamhip {
+namespace {
+
+// steps that the states are kept apart: the backward pass holds TB * P states and as many decays a lane
+constexpr int block_steps(int P) { return P == 8 ? 8 : 16; }
+
+struct ScanArgs {
+  const void *u, *delta, *z, *Bm, *Cm, *dy;
+  const float *A, *D, *bias, *state_in, *d_state_out;
+  void *y, *du, *ddelta, *dz;
+  float *state_out, *kept, *d_state_in;
+  float *ends, *sums, *part, *part_bc;   // workspace
+  const int* lengths;
+  long long ub, ut, deltab, deltat, zb, zt, Bb, Bt, Cb, Ct, yb, yt;
+  long long dyb, dyt, dub, dut, ddeltab, ddeltat, dzb, dzt;
+  int T, C, N, chunk, chunks, softplus;
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+template <int K>
+__device__ __forceinline__ float quad_lane(float v) {
+  return dpp_<K * 0x55>(v);
+}
+
+__device__ __forceinline__ float quad_sum(float v) {
+  v += dpp_<0xB1>(v);
+  return v + dpp_<0x4E>(v);
+}
+
+// v[k] summed over the quad, for the lane whose place in the quad is k
+__device__ __forceinline__ float quad_sum_own(const float (&v)[4], int q) {
+  const bool odd = q & 1, high = q & 2;
+  const float a0 = (odd ? v[1] : v[0]) + dpp_<0xB1>(odd ? v[0] : v[1]);
+  const float a1 = (odd ? v[3] : v[2]) + dpp_<0xB1>(odd ? v[2] : v[3]);
+  return (high ? a1 : a0) + dpp_<0x4E>(high ? a0 : a1);
+}
+
+// ln(1 + e^v); the part of e that the rounding of 1 + e drops is added back, so that small results keep their relative precision
+__device__ __forceinline__ float softplus_(float v, float e) {
+  const float w = 1.0f + e;
+  const float lost = e - (w - 1.0f);
+  return fmaxf(v, 0.0f) + fmaf(log2_(w), kLn2, lost);
+}
+
+struct Lane {
+  int q, c, cc, len, own, b;   // own: the lane's own length, 0 without a channel
+  bool live;
+};
+
+__device__ __forceinline__ Lane scan_lane(const ScanArgs& a) {
+  Lane l;
+  l.q = threadIdx.x & 3;
+  l.c = blockIdx.x * 64 + (threadIdx.x >> 2);
+  l.live = l.c < a.C;
+  l.cc = l.live ? l.c : a.C - 1;   // lanes without a channel read the last one's parameters and have no steps
+  l.b = blockIdx.z;
+  l.len = a.T;
+  if (a.lengths) {
+    const int n = a.lengths[l.b];
+    l.len = n < 0 ? 0 : (n > a.T ? a.T : n);
+  }
+  l.own = l.live ? l.len : 0;
+  return l;
+}
+
+template <int P>
+__device__ __forceinline__ void load_states(const float* p, int N, int q, float (&v)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = q * P + i < N ? p[q * P + i] : 0.0f;
+}
+
+template <int P>
+__device__ __forceinline__ void store_states(float* p, int N, int q, const float (&v)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (q * P + i < N) p[q * P + i] = v[i];
+}
+
+// B and C of steps [t0, t0 + TB) in float32, zeros beyond the sequence's end and beyond N
+template <typename T, int P, int TB>
+struct Staged {
+  static constexpr int kPer = TB * 8 * P / 256 > 0 ? TB * 8 * P / 256 : 1;
+  float v[kPer];
+  __device__ __forceinline__ void load(const ScanArgs& a, const Lane& l, int t0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = i * 256 + threadIdx.x, n = at % (4 * P), which = at / (4 * P) & 1, t = t0 + at / (8 * P);
+      v[i] = 0.0f;
+      if (at < TB * 8 * P && n < a.N && t < l.len) {
+        const T* p = which ? (const T*)a.Cm + l.b * a.Cb + t * a.Ct : (const T*)a.Bm + l.b * a.Bb + t * a.Bt;
+        v[i] = (float)p[n];
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float* sh) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i * 256 + threadIdx.x < TB * 8 * P) sh[i * 256 + threadIdx.x] = v[i];
+  }
+};
+
+template <int P>
+__device__ __forceinline__ void read_states(const float* sh, float (&v)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = sh[i];
+}
+
+// a lane's own steps of a block: t0 + q, t0 + q + 4, ...; zero outside the sequence
+template <typename T, int G>
+__device__ __forceinline__ void load_own(const void* base, long long sb, long long st, const Lane& l, int t0, float (&v)[G]) {
+  const T* p = (const T*)base + l.b * sb + l.cc;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    const int t = t0 + 4 * i + l.q;
+    v[i] = t < l.own ? (float)p[t * st] : 0.0f;
+  }
+}
+
+// STATES: the first pass of a cut sequence: each chunk's end state from zero (the first chunk's from state_in) and its sum of dt
+template <typename T, int P, bool STATES>
+__global__ void __launch_bounds__(256) selective_scan_fwd_kernel(ScanArgs a) {
+  constexpr int TB = block_steps(P), G = TB / 4;
+  __shared__ float bc[2][TB * 8 * P];
+  const Lane l = scan_lane(a);
+  const int chunk = blockIdx.y, t_begin = chunk * a.chunk, t_end = min(t_begin + a.chunk, a.T);
+  const long long bC = (long long)l.b * a.C + l.cc;
+  const long long slots = a.chunks + 1;   // a.ends [B][chunks + 1][C][N]: state_in, then each chunk's end
+  float h[P], A2[P];
+  load_states<P>(a.A + (long long)l.cc * a.N, a.N, l.q, A2);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    A2[i] *= kLog2e;
+    h[i] = 0.0f;
+  }
+  if (STATES || a.chunks == 1) {
+    if (chunk == 0 && a.state_in) load_states<P>(a.state_in + bC * a.N, a.N, l.q, h);
+    if (STATES && chunk == 0 && l.live) store_states<P>(a.ends + ((long long)l.b * slots * a.C + l.c) * a.N, a.N, l.q, h);
+  } else if (chunk == 0) {
+    load_states<P>(a.ends + ((long long)l.b * slots * a.C + l.cc) * a.N, a.N, l.q, h);
+  } else {
+    for (int j = 0; j < chunk; ++j) {
+      const float s = a.sums[((long long)l.b * a.chunks + j) * a.C + l.cc];
+      float e[P];
+      load_states<P>(a.ends + (((long long)l.b * slots + j + 1) * a.C + l.cc) * a.N, a.N, l.q, e);
+#pragma unroll
+      for (int i = 0; i < P; ++i) h[i] = fmaf(exp2_(A2[i] * s), h[i], e[i]);
+    }
+  }
+  const float bias = a.bias ? a.bias[l.cc] : 0.0f, D = a.D ? a.D[l.cc] : 0.0f;
+  const long long nblocks = (a.T + TB - 1) / TB;
+  float dt_sum = 0.0f;
+
+  Staged<T, P, TB> next_bc;
+  float nu[G], nd[G], nz[G];
+  auto fetch = [&](int t0) {
+    next_bc.load(a, l, t0);
+    load_own<T, G>(a.u, a.ub, a.ut, l, t0, nu);
+    load_own<T, G>(a.delta, a.deltab, a.deltat, l, t0, nd);
+    if (!STATES && a.z) load_own<T, G>(a.z, a.zb, a.zt, l, t0, nz);
+  };
+  if (t_begin < t_end) fetch(t_begin);
+  int buf = 0;
+  for (int t0 = t_begin; t0 < t_end; t0 += TB, buf ^= 1) {
+    if (!STATES && a.kept && l.live)
+      store_states<P>(a.kept + (((long long)l.b * nblocks + t0 / TB) * a.C + l.c) * a.N, a.N, l.q, h);
+    next_bc.put(bc[buf]);
+    float u[G], dt[G], x[G], z[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float raw = nd[i] + bias;
+      dt[i] = raw;
+      if (a.softplus) dt[i] = softplus_(raw, exp2_(-kLog2e * fabsf(raw)));
+      if (t0 + 4 * i + l.q >= l.own) dt[i] = 0.0f;
+      u[i] = nu[i];
+      x[i] = dt[i] * u[i];
+      dt_sum += dt[i];
+      if (!STATES && a.z) z[i] = nz[i];
+    }
+    __syncthreads();   // bc[buf] is whole; bc[buf ^ 1] has been read by all
+    if (t0 + TB < t_end) fetch(t0 + TB);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      float inner[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (t0 + 4 * i < l.len) {
+        auto step = [&](auto k) {
+          constexpr int K = decltype(k)::value;
+          const float* sh = bc[buf] + (4 * i + K) * 8 * P + l.q * P;
+          float Bv[P], Cv[P];
+          read_states<P>(sh, Bv);
+          if (!STATES) read_states<P>(sh + 4 * P, Cv);
+          const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x[i]);
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            h[p] = fmaf(exp2_(A2[p] * d), h[p], xv * Bv[p]);
+            if (!STATES) inner[K] = fmaf(h[p], Cv[p], inner[K]);
+          }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+      }
+      if (!STATES) {
+        const int t = t0 + 4 * i + l.q;
+        float v = fmaf(D, u[i], quad_sum_own(inner, l.q));
+        if (a.z) v *= z[i] * sigmoid_(z[i]);
+        if (t >= l.len) v = 0.0f;
+        if (l.live && t < t_end) ((T*)a.y + l.b * a.yb + t * a.yt)[l.c] = (T)v;
+      }
+    }
+  }
+  if (STATES) {
+    if (l.live) {
+      store_states<P>(a.ends + (((long long)l.b * slots + chunk + 1) * a.C + l.c) * a.N, a.N, l.q, h);
+      const float s = quad_sum(dt_sum);
+      if (l.q == 0) a.sums[((long long)l.b * a.chunks + chunk) * a.C + l.c] = s;
+    }
+  } else if (a.state_out && chunk == a.chunks - 1 && l.live) {
+    store_states<P>(a.state_out + bC * a.N, a.N, l.q, h);
+  }
+}
+
+// v[p] (p < P) and w[p] summed over the wave's 16 channels (lanes of equal place in the quad).  Swapping halves (rows) of two
+// registers and adding them sums both at once, half a wave (a row) each; what is left are four channels of a row.
+template <int P>
+__device__ __forceinline__ void channel_sums(float (&v)[2 * P]) {
+  // after the swaps, register r of lane row `row` holds the sum of value 4 r' + order[row]
+  static_assert(P == 1 || P == 2 || P == 4 || P == 8, "");
+  if constexpr (2 * P >= 4) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), false, false);
+      v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), false, false);
+      v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      v[i] += dpp_<0x124>(v[i]);   // row_ror:4
+      v[i] += dpp_<0x128>(v[i]);   // row_ror:8
+    }
+  } else {   // two values: one for each half of the wave, rows added with a further swap
+    auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0]), __float_as_uint(v[1]), false, false);
+    v[0] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0]), __float_as_uint(v[0]), false, false);
+    v[0] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    v[0] += dpp_<0x124>(v[0]);
+    v[0] += dpp_<0x128>(v[0]);
+  }
+}
+
+// what value of v register i of channel_sums() holds in row `row` of the wave
+template <int P>
+__device__ __forceinline__ int channel_sum_index(int i, int row) {
+  if (P == 1) return row >> 1;                       // halves
+  return 4 * i + 2 * (row & 1) + (row >> 1);         // row 0: 4i, row 1: 4i + 2, row 2: 4i + 1, row 3: 4i + 3
+}
+
+// CARRY: the first pass of a cut sequence: the gradient that each chunk by itself hands to the state in front of it
+template <typename T, int P, bool CARRY>
+__global__ void __launch_bounds__(256, 2) selective_scan_bwd_kernel(ScanArgs a) {
+  constexpr int TB = block_steps(P), G = TB / 4;
+  __shared__ float bc[TB * 8 * P];
+  __shared__ float bc_grad[CARRY ? 1 : 4][CARRY ? 1 : TB * 8 * P];
+  const Lane l = scan_lane(a);
+  const int wave = threadIdx.x >> 6;
+  const int chunk = blockIdx.y, t_begin = chunk * a.chunk, t_end = min(t_begin + a.chunk, a.T);
+  const long long bC = (long long)l.b * a.C + l.cc;
+  float A2[P], g[P], dA[P];
+  load_states<P>(a.A + (long long)l.cc * a.N, a.N, l.q, A2);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    A2[i] *= kLog2e;
+    g[i] = 0.0f;
+    dA[i] = 0.0f;
+  }
+  if (!CARRY || chunk == a.chunks - 1)
+    if (a.d_state_out) load_states<P>(a.d_state_out + bC * a.N, a.N, l.q, g);
+  if (!CARRY)
+    for (int j = a.chunks - 1; j > chunk; --j) {   // the last chunk's own carry holds d_state_out already
+      const float s = a.sums[((long long)l.b * a.chunks + j) * a.C + l.cc];
+      float e[P];
+      load_states<P>(a.ends + (((long long)l.b * a.chunks + j) * a.C + l.cc) * a.N, a.N, l.q, e);
+#pragma unroll
+      for (int i = 0; i < P; ++i) g[i] = j == a.chunks - 1 ? e[i] : fmaf(exp2_(A2[i] * s), g[i], e[i]);
+    }
+  const float bias = a.bias ? a.bias[l.cc] : 0.0f, D = a.D ? a.D[l.cc] : 0.0f;
+  const long long nblocks = (a.T + TB - 1) / TB;
+  const int groups = gridDim.x;
+  float dt_sum = 0.0f, dD = 0.0f, dbias = 0.0f;
+
+  for (int t0 = t_begin + (t_end - 1 - t_begin) / TB * TB; t0 >= t_begin && t_begin < t_end; t0 -= TB) {
+    Staged<T, P, TB> stage;
+    stage.load(a, l, t0);
+    float u[G], raw[G], z[G], dy[G], dt[G], e[G], slope[G];
+    load_own<T, G>(a.u, a.ub, a.ut, l, t0, u);
+    load_own<T, G>(a.delta, a.deltab, a.deltat, l, t0, raw);
+    load_own<T, G>(a.dy, a.dyb, a.dyt, l, t0, dy);
+    if (a.z) load_own<T, G>(a.z, a.zb, a.zt, l, t0, z);
+    float h[P];
+    if (!CARRY) load_states<P>(a.kept + (((long long)l.b * nblocks + t0 / TB) * a.C + l.cc) * a.N, a.N, l.q, h);
+    __syncthreads();   // the previous block's bc and bc_grad have been read
+    stage.put(bc);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const bool in = t0 + 4 * i + l.q < l.own;
+      const float r = raw[i] + bias;
+      dt[i] = r;
+      slope[i] = 1.0f;
+      if (a.softplus) {
+        const float x = exp2_(-kLog2e * fabsf(r));
+        dt[i] = softplus_(r, x);
+        slope[i] = (r >= 0.0f ? 1.0f : x) * rcp_(1.0f + x);
+      }
+      if (!in) dt[i] = 0.0f;
+      e[i] = dy[i];
+      if (a.z) e[i] *= z[i] * sigmoid_(z[i]);
+      if (!in) e[i] = 0.0f;
+      dt_sum += dt[i];
+    }
+    __syncthreads();
+    if (CARRY) {
+#pragma unroll
+      for (int i = G - 1; i >= 0; --i) {
+        auto step = [&](auto k) {
+          constexpr int K = decltype(k)::value;
+          const float* sh = bc + (4 * i + K) * 8 * P + l.q * P;
+          float Cv[P];
+          read_states<P>(sh + 4 * P, Cv);
+          const float d = quad_lane<K>(dt[i]), ev = quad_lane<K>(e[i]);
+#pragma unroll
+          for (int p = 0; p < P; ++p) g[p] = fmaf(ev, Cv[p], g[p]) * exp2_(A2[p] * d);
+        };
+        step(std::integral_constant<int, 3>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 0>{});
+      }
+      continue;
+    }
+    float hs[TB][P], as[TB][P];   // the state in front of each step, and its decay
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float x = dt[i] * u[i];
+      auto step = [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        const float* sh = bc + (4 * i + K) * 8 * P + l.q * P;
+        float Bv[P];
+        read_states<P>(sh, Bv);
+        const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          hs[4 * i + K][p] = h[p];
+          as[4 * i + K][p] = exp2_(A2[p] * d);
+          h[p] = fmaf(as[4 * i + K][p], h[p], xv * Bv[p]);
+        }
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+      step(std::integral_constant<int, 2>{});
+      step(std::integral_constant<int, 3>{});
+    }
+#pragma unroll
+    for (int i = G - 1; i >= 0; --i) {
+      const float x = dt[i] * u[i];
+      float inner[4], gb[4], qa[4];
+      auto step = [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        const float* sh = bc + (4 * i + K) * 8 * P + l.q * P;
+        float Bv[P], Cv[P], v[2 * P];
+        read_states<P>(sh, Bv);
+        read_states<P>(sh + 4 * P, Cv);
+        const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x), ev = quad_lane<K>(e[i]);
+        float s_in = 0.0f, s_gb = 0.0f, s_qa = 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          g[p] = fmaf(ev, Cv[p], g[p]);
+          s_in = fmaf(h[p], Cv[p], s_in);
+          v[P + p] = ev * h[p];
+          v[p] = g[p] * xv;
+          s_gb = fmaf(g[p], Bv[p], s_gb);
+          g[p] *= as[4 * i + K][p];
+          h[p] = hs[4 * i + K][p];
+          const float q = g[p] * h[p];
+          dA[p] = fmaf(q, d, dA[p]);
+          s_qa = fmaf(q, A2[p], s_qa);
+        }
+        inner[K] = s_in;
+        gb[K] = s_gb;
+        qa[K] = s_qa;
+        channel_sums<P>(v);
+        constexpr int R = P >= 2 ? P / 2 : 1;
+        if ((threadIdx.x & 12) == 0) {   // the first channel of each row
+          const int row = threadIdx.x >> 4 & 3;
+          float* out = bc_grad[wave] + (4 * i + K) * 8 * P;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int at = channel_sum_index<P>(r, row);   // below P: dB of state at, else dC of state at - P
+            out[(at >= P ? 4 * P + at - P : at) + l.q * P] = v[r];
+          }
+        }
+      };
+      step(std::integral_constant<int, 3>{});
+      step(std::integral_constant<int, 2>{});
+      step(std::integral_constant<int, 1>{});
+      step(std::integral_constant<int, 0>{});
+      const int t = t0 + 4 * i + l.q;
+      const float in_sum = quad_sum_own(inner, l.q), gb_sum = quad_sum_own(gb, l.q), qa_sum = quad_sum_own(qa, l.q);
+      const bool in = t < l.len;
+      float du = fmaf(gb_sum, dt[i], D * e[i]);
+      float dd = fmaf(gb_sum, u[i], qa_sum * kLn2) * slope[i];
+      if (!in) du = dd = 0.0f;
+      dD = fmaf(e[i], u[i], dD);
+      dbias += dd;
+      if (l.live && t < t_end) {
+        ((T*)a.du + l.b * a.dub + t * a.dut)[l.c] = (T)du;
+        ((T*)a.ddelta + l.b * a.ddeltab + t * a.ddeltat)[l.c] = (T)dd;
+        if (a.dz) {
+          const float s = sigmoid_(z[i]);
+          float dz = dy[i] * fmaf(D, u[i], in_sum) * s * fmaf(z[i], 1.0f - s, 1.0f);
+          if (!in) dz = 0.0f;
+          ((T*)a.dz + l.b * a.dzb + t * a.dzt)[l.c] = (T)dz;
+        }
+      }
+    }
+    __syncthreads();
+    // part_bc [B][T][groups][2][4 P]
+    for (int at = threadIdx.x; at < TB * 8 * P; at += 256) {
+      const int t = t0 + at / (8 * P);
+      if (t < t_end)
+        a.part_bc[(((long long)l.b * a.T + t) * groups + blockIdx.x) * 8 * P + at % (8 * P)] =
+            (bc_grad[0][at] + bc_grad[1][at]) + (bc_grad[2][at] + bc_grad[3][at]);
+    }
+  }
+  if (CARRY) {
+    if (l.live) {
+      store_states<P>(a.ends + (((long long)l.b * a.chunks + chunk) * a.C + l.c) * a.N, a.N, l.q, g);
+      const float s = quad_sum(dt_sum);
+      if (l.q == 0) a.sums[((long long)l.b * a.chunks + chunk) * a.C + l.c] = s;
+    }
+    return;
+  }
+  dD = quad_sum(dD);
+  dbias = quad_sum(dbias);
+  if (l.live) {
+    if (a.d_state_in && chunk == 0) store_states<P>(a.d_state_in + bC * a.N, a.N, l.q, g);
+    // part [B * chunks][C * N of dA, C of dD, C of the bias]
+    float* part = a.part + ((long long)l.b * a.chunks + chunk) * a.C * (a.N + 2);
+    store_states<P>(part + (long long)l.c * a.N, a.N, l.q, dA);
+    if (l.q == 0) {
+      part[(long long)a.C * a.N + l.c] = dD;
+      part[(long long)a.C * (a.N + 1) + l.c] = dbias;
+    }
+  }
+}
+
+// dB and dC from the parts of the channel groups; a thread a value
+template <typename T>
+__global__ void __launch_bounds__(256) selective_scan_bc_kernel(const float* __restrict__ part, int groups, int np, int N, long long steps,
+                                                                int T_, const int* __restrict__ lengths, T* dB, T* dC, long long dBb,
+                                                                long long dBt, long long dCb, long long dCt) {
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long step = at / (2 * np);
+  if (step >= steps) return;
+  const int v = (int)(at - step * 2 * np), which = v / np, n = v - which * np;
+  if (n >= N) return;
+  const int b = (int)(step / T_), t = (int)(step - (long long)b * T_);
+  float s = 0.0f;
+  for (int g = 0; g < groups; ++g) s += part[(step * groups + g) * 2 * np + v];
+  if (lengths && t >= lengths[b]) s = 0.0f;
+  if (which)
+    dC[b * dCb + t * dCt + n] = (T)s;
+  else
+    dB[b * dBb + t * dBt + n] = (T)s;
+}
+
+struct ScanGradients {
+  float *dA, *dD, *dbias;
+  int C, N;
+  __device__ void operator()(int i, float v) const {
+    if (i < C * N)
+      dA[i] = v;
+    else if (i < C * (N + 1)) {
+      if (dD) dD[i - C * N] = v;
+    } else if (dbias)
+      dbias[i - C * (N + 1)] = v;
+  }
+};
+
+struct ScanShape {
+  int P, groups, chunk, chunks;
+};
+
+// Chunks, where the channels alone give fewer waves than two a SIMD (2048): the first pass costs more than half of the second,
+// so no more of them than that takes, and none of under 64 steps.
+ScanShape scan_shape(int B, int T, int C, int N) {
+  ScanShape s;
+  s.P = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
+  s.groups = (C + 63) / 64;
+  const long long waves = (long long)B * s.groups * 4;
+  long long chunks = (2048 + waves - 1) / waves;
+  if (chunks > T / 64) chunks = T / 64;
+  if (chunks < 1) chunks = 1;
+  const int per = (int)((T + chunks - 1) / chunks);
+  s.chunk = (per + 15) / 16 * 16;
+  if (s.chunk < 16) s.chunk = 16;
+  s.chunks = T > 0 ? (T + s.chunk - 1) / s.chunk : 1;
+  return s;
+}
+
+template <typename T, int P>
+int scan_fwd(const ScanArgs& a, dim3 grid, hipStream_t s) {
+  if (a.chunks > 1) hipLaunchKernelGGL((selective_scan_fwd_kernel<T, P, true>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((selective_scan_fwd_kernel<T, P, false>), grid, dim3(256), 0, s, a);
+  SLAMHIP_HIP(hipGetLastError());
+  return SLAMHIP_OK;
+}
+
+template <typename T, int P>
+int scan_bwd(const ScanArgs& a, dim3 grid, hipStream_t s) {
+  if (a.chunks > 1) hipLaunchKernelGGL((selective_scan_bwd_kernel<T, P, true>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((selective_scan_bwd_kernel<T, P, false>), grid, dim3(256), 0, s, a);
+  SLAMHIP_HIP(hipGetLastError());
+  return SLAMHIP_OK;
+}
+
+}  // namespace
+}  // namespace slamhip
+
+using namespace slamhip;
+
+#define SLAMHIP_SCAN_DISPATCH(FN, P, ...)                     \
+  (dtype == SLAMHIP_BF16 ? ((P) == 1   ? FN<__bf16, 1>(__VA_ARGS__)  \
+                            : (P) == 2 ? FN<__bf16, 2>(__VA_ARGS__)  \
+                            : (P) == 4 ? FN<__bf16, 4>(__VA_ARGS__)  \
+                                       : FN<__bf16, 8>(__VA_ARGS__)) \
+                         : ((P) == 1   ? FN<float, 1>(__VA_ARGS__)   \
+                            : (P) == 2 ? FN<float, 2>(__VA_ARGS__)   \
+                            : (P) == 4 ? FN<float, 4>(__VA_ARGS__)   \
+                                       : FN<float, 8>(__VA_ARGS__)))
+
+#define SLAMHIP_SCAN_SIZES(name)                                                                                               \
+  SLAMHIP_REQUIRE(B >= 0 && T >= 0 && C > 0 && N > 0 && N <= 32 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG, \
+                  name ": need C >= 1, 1 <= N <= 32 and a known type");                                                        \
+  SLAMHIP_REQUIRE(B <= 65535 && T <= (1 << 20) && C <= (1 << 20), SLAMHIP_E_SIZE, name ": at most 65535 sequences, 2^20 steps and channels")
+
+extern "C" {
+
+size_t slamhip_selective_scan_kept_floats(int B, int T, int C, int N) {
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  const int tb = block_steps(scan_shape(B, T, C, N).P);
+  return (size_t)B * ((T + tb - 1) / tb) * C * N;
+}
+
+size_t slamhip_selective_scan_fwd_workspace_bytes(int B, int T, int C, int N) {
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  const ScanShape g = scan_shape(B, T, C, N);
+  if (g.chunks == 1) return 0;
+  return ((size_t)B * (g.chunks + 1) * C * N + (size_t)B * g.chunks * C) * sizeof(float);
+}
+
+int slamhip_selective_scan_fwd(const void* u, const void* delta, const void* z, const void* Bm, const void* Cm, const long long* strides,
+                               const float* A, const float* D, const float* delta_bias, const float* state_in, const int32_t* lengths,
+                               int B, int T, int C, int N, int softplus, int dtype, void* y, float* state_out, float* kept_states,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  SLAMHIP_SCAN_SIZES("selective_scan_fwd");
+  if (B == 0 || (T == 0 && !state_out)) return SLAMHIP_OK;
+  SLAMHIP_REQUIRE(A && strides && (T == 0 || (u && delta && Bm && Cm && y)), SLAMHIP_E_ARG, "selective_scan_fwd: null pointer");
+  SLAMHIP_REQUIRE(workspace_bytes >= slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N) &&
+                      (workspace || slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N) == 0),
+                  SLAMHIP_E_ARG, "selective_scan_fwd: workspace too small");
+  const ScanShape g = scan_shape(B, T, C, N);
+  ScanArgs a{};
+  a.u = u, a.delta = delta, a.z = z, a.Bm = Bm, a.Cm = Cm, a.A = A, a.D = D, a.bias = delta_bias, a.state_in = state_in;
+  a.y = y, a.state_out = state_out, a.kept = kept_states, a.lengths = lengths;
+  a.ub = strides[0], a.ut = strides[1], a.deltab = strides[2], a.deltat = strides[3], a.zb = strides[4], a.zt = strides[5];
+  a.Bb = strides[6], a.Bt = strides[7], a.Cb = strides[8], a.Ct = strides[9], a.yb = strides[10], a.yt = strides[11];
+  a.T = T, a.C = C, a.N = N, a.chunk = g.chunk, a.chunks = g.chunks, a.softplus = softplus;
+  a.ends = (float*)workspace;
+  a.sums = a.ends + (size_t)B * (g.chunks + 1) * C * N;
+  return SLAMHIP_SCAN_DISPATCH(scan_fwd, g.P, a, dim3(g.groups, g.chunks, B), (hipStream_t)stream);
+}
+
+size_t slamhip_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N) {
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  const ScanShape g = scan_shape(B, T, C, N);
+  const size_t carry = g.chunks > 1 ? (size_t)B * g.chunks * C * (N + 1) : 0;
+  return (carry + (size_t)B * g.chunks * C * (N + 2) + (size_t)B * T * g.groups * 8 * g.P) * sizeof(float);
+}
+
+int slamhip_selective_scan_bwd(const void* dy, const void* u, const void* delta, const void* z, const void* Bm, const void* Cm,
+                               const long long* strides, const float* A, const float* D, const float* delta_bias,
+                               const float* kept_states, const float* d_state_out, const int32_t* lengths, int B, int T, int C, int N,
+                               int softplus, int dtype, void* du, void* ddelta, void* dz, void* dB, void* dC, float* dA, float* dD,
+                               float* d_delta_bias, float* d_state_in, void* workspace, size_t workspace_bytes, void* stream) {
+  SLAMHIP_SCAN_SIZES("selective_scan_bwd");
+  const bool work = B > 0 && T > 0;
+  SLAMHIP_REQUIRE(dA && (!work || (A && strides && dy && u && delta && Bm && Cm && kept_states && du && ddelta && dB && dC && workspace)),
+                  SLAMHIP_E_ARG, "selective_scan_bwd: null pointer");
+  SLAMHIP_REQUIRE(!work || !z == !dz, SLAMHIP_E_ARG, "selective_scan_bwd: z and dz come together");
+  SLAMHIP_REQUIRE(work || B == 0 || !d_state_in, SLAMHIP_E_ARG, "selective_scan_bwd: no steps");
+  SLAMHIP_REQUIRE(workspace_bytes >= slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N), SLAMHIP_E_ARG, "selective_scan_bwd: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  const ScanShape g = scan_shape(B, T, C, N);
+  float* part = (float*)workspace;
+  SLAMHIP_REQUIRE((long long)C * (N + 2) <= 0x7fffffffLL, SLAMHIP_E_SIZE, "selective_scan_bwd: too many parameters");
+  if (work) {
+    ScanArgs a{};
+    a.u = u, a.delta = delta, a.z = z, a.Bm = Bm, a.Cm = Cm, a.dy = dy, a.A = A, a.D = D, a.bias = delta_bias;
+    a.d_state_out = d_state_out, a.kept = const_cast<float*>(kept_states), a.lengths = lengths;
+    a.du = du, a.ddelta = ddelta, a.dz = dz, a.d_state_in = d_state_in;
+    a.dyb = strides[0], a.dyt = strides[1], a.ub = strides[2], a.ut = strides[3], a.deltab = strides[4], a.deltat = strides[5];
+    a.zb = strides[6], a.zt = strides[7], a.Bb = strides[8], a.Bt = strides[9], a.Cb = strides[10], a.Ct = strides[11];
+    a.dub = strides[12], a.dut = strides[13], a.ddeltab = strides[14], a.ddeltat = strides[15], a.dzb = strides[16], a.dzt = strides[17];
+    a.T = T, a.C = C, a.N = N, a.chunk = g.chunk, a.chunks = g.chunks, a.softplus = softplus;
+    a.part = part;
+    a.part_bc = part + (size_t)B * g.chunks * C * (N + 2);
+    a.ends = a.part_bc + (size_t)B * T * g.groups * 8 * g.P;
+    a.sums = a.ends + (size_t)B * g.chunks * C * N;
+    const int rc = SLAMHIP_SCAN_DISPATCH(scan_bwd, g.P, a, dim3(g.groups, g.chunks, B), s);
+    if (rc != SLAMHIP_OK) return rc;
+    const long long values = (long long)B * T * 8 * g.P, blocks = (values + 255) / 256;
+    SLAMHIP_REQUIRE(blocks < (1 << 24), SLAMHIP_E_SIZE, "selective_scan_bwd: too many steps");
+    if (dtype == SLAMHIP_BF16)
+      hipLaunchKernelGGL((selective_scan_bc_kernel<__bf16>), dim3((unsigned)blocks), dim3(256), 0, s, a.part_bc, g.groups, 4 * g.P, N,
+                         (long long)B * T, T, lengths, (__bf16*)dB, (__bf16*)dC, strides[18], strides[19], strides[20], strides[21]);
+    else
+      hipLaunchKernelGGL((selective_scan_bc_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, s, a.part_bc, g.groups, 4 * g.P, N,
+                         (long long)B * T, T, lengths, (float*)dB, (float*)dC, strides[18], strides[19], strides[20], strides[21]);
+    SLAMHIP_HIP(hipGetLastError());
+  }
+  SLAMHIP_HIP(column_sums(part, work ? (long long)B * g.chunks : 0, C * (N + 2), ScanGradients{dA, dD, d_delta_bias, C, N}, s));
+  return SLAMHIP_OK;
+}
+
+}  // extern "C"

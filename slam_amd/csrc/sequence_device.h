@@ -1,0 +1,94 @@
+// Device helpers of the sequence-layer kernels (rms_norm.hip, causal_conv.hip, selective_scan.hip, gemm_fp8.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+// these kernels are compared with tolerances, not bit for bit: products and sums may contract to fma
+#pragma clang fp contract(fast)
+
+namespace slamhip {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// Eight consecutive elements of a row, at the element's own alignment: gfx950 takes unaligned global accesses, so rows of odd
+// length and views at odd offsets use the same 16-byte loads as aligned ones.
+template <typename T>
+struct Packed8;
+template <>
+struct Packed8<float> {
+  typedef f32x8 __attribute__((aligned(4))) type;
+};
+template <>
+struct Packed8<__bf16> {
+  typedef bf16x8 __attribute__((aligned(2))) type;
+};
+
+// valid >= 8: one vector access; fewer: element by element, the rest zero
+template <typename T>
+__device__ __forceinline__ f32x8 load8(const T* p, int valid) {
+  f32x8 v;
+  if (valid >= 8) {
+    const typename Packed8<T>::type raw = *reinterpret_cast<const typename Packed8<T>::type*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? (float)p[i] : 0.0f;
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, f32x8 v, int valid) {
+  if (valid >= 8) {
+    typename Packed8<T>::type raw;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = (T)v[i];
+    *reinterpret_cast<typename Packed8<T>::type*>(p) = raw;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) p[i] = (T)v[i];
+  }
+}
+
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float log2_(float v) { return __builtin_amdgcn_logf(v); }
+__device__ __forceinline__ float rcp_(float v) { return __builtin_amdgcn_rcpf(v); }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// 1 / (1 + e^-v): 0 and 1 at the far ends, NaN stays NaN
+__device__ __forceinline__ float sigmoid_(float v) { return rcp_(1.0f + exp2_(-kLog2e * v)); }
+
+// out(c, sum over parts of part[p][c]), in an order that depends on the sizes alone
+template <typename Out>
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, long long parts, int columns, Out out) {
+  __shared__ float sh[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
+  float s = 0.0f;
+  if (c < columns)
+    for (long long p = ty; p < parts; p += 32) s += part[p * columns + c];
+  sh[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < columns) {
+    s = 0.0f;
+    for (int i = 0; i < 32; ++i) s += sh[i][tx];
+    out(c, s);
+  }
+}
+
+template <typename Out>
+hipError_t column_sums(const float* part, long long parts, int columns, Out out, hipStream_t s) {
+  hipLaunchKernelGGL((column_sum_kernel<Out>), dim3((columns + 31) / 32), dim3(1024), 0, s, part, parts, columns, out);
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace slamhip

@@ -1,0 +1,240 @@
+"""Typed wrappers of the sequence-layer entry points of libslamhip.so: root-mean-square
+norm, 8-bit operands and their product, short causal convolution, selective scan
+(csrc/rms_norm.hip, gemm_fp8.hip, causal_conv.hip, selective_scan.hip).
+
+As in encoder_ops the caller brings GPU tensors for inputs and outputs, every call is
+checked on the host and launches on the current stream (of the tensors' device), and
+there is no autograd: a backward pass is a call of its own.  A refused call raises
+ValueError and launches nothing.  Activations are float32 or bfloat16, parameters,
+statistics and states float32.  Workspaces are torch allocations of the call.
+"""
+import ctypes
+
+import torch
+
+from .. import capi
+from .encoder_ops import BF16, F32
+
+FP8 = torch.float8_e4m3fn
+_DTYPE = {F32: 0, BF16: 1}
+
+
+def _launch(device, name, *args):
+    lib = capi.load()
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            capi.check(getattr(lib, name)(*args, capi.current_stream()), name)
+    else:
+        capi.check(getattr(lib, name)(*args, capi.current_stream()), name)
+
+
+def _bad(what, t, want):
+    got = "None" if t is None else "%s %s on %s, strides %s" % (t.dtype, tuple(t.shape), t.device, t.stride())
+    raise ValueError("%s: expected %s, got %s" % (what, want, got))
+
+
+def _flat(t, dtype, shape, device, what):
+    """A contiguous tensor of this type and shape on `device`; its address."""
+    if t is None or t.dtype is not dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        _bad(what, t, "a contiguous %s tensor %s on %s" % (dtype, shape, device))
+    return t.data_ptr()
+
+
+def _opt(t, dtype, shape, device, what):
+    return None if t is None else _flat(t, dtype, shape, device, what)
+
+
+def _matrix(t, what):
+    """(rows, columns, type code, device) of a contiguous float32 or bfloat16 GPU matrix."""
+    if t.dim() != 2 or t.dtype not in _DTYPE or not t.is_cuda or not t.is_contiguous() or t.shape[1] == 0:
+        _bad(what, t, "a contiguous float32 or bfloat16 GPU matrix with columns")
+    return t.shape[0], t.shape[1], _DTYPE[t.dtype], t.device
+
+
+def _seq(t, dtype, shape, device, what, out=False):
+    """A sequence [B, T, C] of this type with unit stride over C; an output's rows may not overlap."""
+    if t is None or t.dtype is not dtype or tuple(t.shape) != shape or t.device != device:
+        _bad(what, t, "a %s tensor %s on %s" % (dtype, shape, device))
+    (B, T, C), (sb, st, sc) = shape, t.stride()
+    if sc != 1 and C > 1:
+        _bad(what, t, "unit stride over the last axis")
+    if out and ((T > 1 and st < C) or (B > 1 and sb < C) or (B > 1 and T > 1 and sb < (T - 1) * st + C and st < (B - 1) * sb + C)):
+        _bad(what, t, "rows that do not overlap")
+    return t.data_ptr()
+
+
+def _sequence(t, what):
+    """(B, T, C, type, device) of a float32 or bfloat16 GPU tensor [B, T, C]."""
+    if t.dim() != 3 or t.dtype not in _DTYPE or not t.is_cuda or t.shape[2] == 0:
+        _bad(what, t, "a float32 or bfloat16 GPU tensor [B, T, C] with channels")
+    B, T, C = t.shape
+    return B, T, C, t.dtype, t.device
+
+
+def _strides(*ts):
+    v = []
+    for t in ts:
+        v += (0, 0) if t is None else t.stride()[:2]
+    return (ctypes.c_longlong * len(v))(*v)
+
+
+def _apart(outs, ins):
+    """No output begins where an input does: runs of a sequence are worked on at once."""
+    taken = {t.data_ptr() for t in ins if t is not None and t.numel()}
+    for t in outs:
+        if t is not None and t.numel() and t.data_ptr() in taken:
+            raise ValueError("an output is one of the inputs")
+
+
+def rms_norm_fwd(x, weight, eps, y=None, residual=None, sum_out=None, y8=None, scales=None, rstd=None):
+    """s = x + residual (rounded to x's type, written to sum_out), y = s * (mean(s^2) + eps)^-1/2 * weight over the rows
+    of x [rows, C], C <= 16384.  Any of y, sum_out and the pair y8 (e4m3) / scales (float32 [rows, ceil(C / 128)]) may be asked
+    for; the 8-bit values are those of the unrounded y / scale, scale = max(max|y| / 448, 2^-100) of 128 values.  rstd
+    (float32 [rows]) is kept for rms_norm_bwd.  y and sum_out may be x or residual itself."""
+    rows, C, dt, dev = _matrix(x, "x")
+    _launch(dev, "slamhip_rms_norm_fwd", x.data_ptr(), _opt(residual, x.dtype, (rows, C), dev, "residual"),
+            _flat(weight, F32, (C,), dev, "weight"), eps, rows, C, dt, _opt(sum_out, x.dtype, (rows, C), dev, "sum_out"),
+            _opt(y, x.dtype, (rows, C), dev, "y"), _opt(y8, FP8, (rows, C), dev, "y8"),
+            _opt(scales, F32, (rows, (C + 127) // 128), dev, "scales"), _opt(rstd, F32, (rows,), dev, "rstd"))
+
+
+def rms_norm_bwd(dy, sum_, weight, rstd, dx, dweight, d_sum=None):
+    """Gradients of rms_norm_fwd: dx (of x and of residual alike) and dweight from dy, from sum_ (sum_out of the forward
+    pass, or its x when it had no residual) and from d_sum, the gradient that arrives at sum_out.  dx may be dy or d_sum."""
+    rows, C, dt, dev = _matrix(sum_, "sum")
+    lib = capi.load()
+    nbytes = lib.slamhip_rms_norm_bwd_workspace_bytes(rows, C)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "slamhip_rms_norm_bwd", _flat(dy, sum_.dtype, (rows, C), dev, "dy"), sum_.data_ptr(),
+            _flat(weight, F32, (C,), dev, "weight"), _flat(rstd, F32, (rows,), dev, "rstd"),
+            _opt(d_sum, sum_.dtype, (rows, C), dev, "d_sum"), rows, C, dt, _flat(dx, sum_.dtype, (rows, C), dev, "dx"),
+            _flat(dweight, F32, (C,), dev, "dweight"), ws.data_ptr(), nbytes)
+
+
+def quantize_fp8(x, q, scales):
+    """x [rows, C] -> e4m3 q and a float32 scale for each 128 consecutive values of a row, scales [rows, ceil(C / 128)]."""
+    rows, C, dt, dev = _matrix(x, "x")
+    _launch(dev, "slamhip_quantize_fp8", x.data_ptr(), rows, C, dt, _flat(q, FP8, (rows, C), dev, "q"),
+            _flat(scales, F32, (rows, (C + 127) // 128), dev, "scales"))
+
+
+def quantize_fp8_blocks(x, q, scales):
+    """quantize_fp8 with a scale for each 128 x 128 block: scales [ceil(R / 128), ceil(C / 128)] (the product's weights)."""
+    R, C, dt, dev = _matrix(x, "x")
+    _launch(dev, "slamhip_quantize_fp8_blocks", x.data_ptr(), R, C, dt, _flat(q, FP8, (R, C), dev, "q"),
+            _flat(scales, F32, ((R + 127) // 128, (C + 127) // 128), dev, "scales"))
+
+
+def gemm_nt_fp8(a8, a_scales, b8, b_scales, out):
+    """out [M, N] (bfloat16) = a8 . b8^T of e4m3 operands a8 [M, K], b8 [N, K], where each 128 values of an a8 row have
+    a scale, a_scales [M, ceil(K / 128)], and each 128 x 128 block of b8 one, b_scales [ceil(N / 128), ceil(K / 128)]: what
+    quantize_fp8 (or rms_norm_fwd) and quantize_fp8_blocks write.  K a multiple of 16."""
+    if out.dim() != 2 or not out.is_cuda or a8.dim() != 2 or a8.shape[1] == 0:
+        _bad("out", out, "a bfloat16 GPU matrix and operands with columns")
+    (M, N), K, dev = out.shape, a8.shape[1], out.device
+    kb = (K + 127) // 128
+    if K % 16 or a8.data_ptr() % 16 or b8.data_ptr() % 16:
+        raise ValueError("gemm_nt_fp8: K must be a multiple of 16 and the operands 16-byte aligned, got K = %d" % K)
+    _launch(dev, "slamhip_gemm_nt_fp8", _flat(a8, FP8, (M, K), dev, "a8"), _flat(a_scales, F32, (M, kb), dev, "a_scales"),
+            _flat(b8, FP8, (N, K), dev, "b8"), _flat(b_scales, F32, ((N + 127) // 128, kb), dev, "b_scales"), M, N, K,
+            _flat(out, BF16, (M, N), dev, "out"))
+
+
+def _taps(weight, C, device):
+    if weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
+        _bad("weight", weight, "[%d, K] with 2 <= K <= 4" % C)
+    return _flat(weight, F32, (C, weight.shape[1]), device, "weight"), weight.shape[1]
+
+
+def causal_conv_fwd(x, weight, bias, y, state_in=None, state_out=None, lengths=None, silu=True):
+    """Convolution over time of x [B, T, C] with one filter a channel, weight [C, K], 2 <= K <= 4:
+    pre[t] = bias + sum_k weight[:, k] xp[t + k] with xp = state_in [B, K - 1, C] (None: zeros) followed by x, and
+    y = pre * sigmoid(pre) (pre with silu=False).  state_out receives the last K - 1 rows of xp, to be state_in of the call that
+    continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths (int32 [B]) bounds each sequence:
+    rows behind it are not used and are zero in y.  x and y may be views with any strides over B and T."""
+    B, T, C, dt, dev = _sequence(x, "x")
+    _seq(x, dt, (B, T, C), dev, "x")
+    w, K = _taps(weight, C, dev)
+    _apart((y, state_out), (x,))
+    _apart((y,), (state_in,))
+    _launch(dev, "slamhip_causal_conv_fwd", x.data_ptr(), _strides(x, y), w, _opt(bias, F32, (C,), dev, "bias"),
+            _opt(state_in, dt, (B, K - 1, C), dev, "state_in"), _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K,
+            int(silu), _DTYPE[dt], _seq(y, dt, (B, T, C), dev, "y", out=True), _opt(state_out, dt, (B, K - 1, C), dev, "state_out"))
+
+
+def causal_conv_bwd(dy, x, weight, bias, dx, dweight, dbias=None, state_in=None, d_state_in=None, d_state_out=None, lengths=None,
+                    silu=True):
+    """Gradients of causal_conv_fwd (same x, weight, bias, state_in, lengths, silu): dx, dweight, dbias and d_state_in from dy
+    and from d_state_out, the gradient that arrives at state_out."""
+    B, T, C, dt, dev = _sequence(x, "x")
+    _seq(x, dt, (B, T, C), dev, "x")
+    w, K = _taps(weight, C, dev)
+    _apart((dx, d_state_in), (dy, x, state_in, d_state_out))
+    lib = capi.load()
+    nbytes = lib.slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "slamhip_causal_conv_bwd", _seq(dy, dt, (B, T, C), dev, "dy"), x.data_ptr(), _strides(dy, x, dx), w,
+            _opt(bias, F32, (C,), dev, "bias"), _opt(state_in, dt, (B, K - 1, C), dev, "state_in"),
+            _opt(d_state_out, dt, (B, K - 1, C), dev, "d_state_out"), _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K,
+            int(silu), _DTYPE[dt], _seq(dx, dt, (B, T, C), dev, "dx", out=True), _flat(dweight, F32, (C, K), dev, "dweight"),
+            _opt(dbias, F32, (C,), dev, "dbias"), _opt(d_state_in, dt, (B, K - 1, C), dev, "d_state_in"), ws.data_ptr(), nbytes)
+
+
+def selective_scan_kept_states(B, T, C, N, device):
+    """The buffer in which selective_scan_fwd keeps states for selective_scan_bwd (every 16 steps, 8 for N > 16)."""
+    return torch.empty(capi.load().slamhip_selective_scan_kept_floats(B, T, C, N), dtype=F32, device=device)
+
+
+def _scan_inputs(u, delta, A, Bm, Cm, z):
+    B, T, C, dt, dev = _sequence(u, "u")
+    if A.dim() != 2 or not 1 <= A.shape[1] <= 32:
+        _bad("A", A, "[%d, N] with 1 <= N <= 32" % C)
+    N = A.shape[1]
+    ptrs = (_seq(u, dt, (B, T, C), dev, "u"), _seq(delta, dt, (B, T, C), dev, "delta"),
+            None if z is None else _seq(z, dt, (B, T, C), dev, "z"), _seq(Bm, dt, (B, T, N), dev, "Bm"),
+            _seq(Cm, dt, (B, T, N), dev, "Cm"))
+    return B, T, C, N, dt, dev, ptrs
+
+
+def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, softplus=True, state_in=None, state_out=None,
+                       kept_states=None, lengths=None):
+    """dt = softplus(delta + delta_bias), h_t = exp(dt A) h_{t-1} + dt u Bm, y = (Cm . h_t + D u) z / (1 + e^-z) over the steps of
+    u, delta, z, y [B, T, C], A [C, N], Bm, Cm [B, T, N], N <= 32.  D and delta_bias [C] and the gate z are optional; softplus=False
+    takes delta + delta_bias as it is.  state_in [B, C, N] (None: zeros) is h before the first step and state_out h after the last,
+    to be state_in of the call that continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths
+    (int32 [B]) bounds each sequence: rows behind it are not used and are zero in y.  kept_states (selective_scan_kept_states)
+    is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T."""
+    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z)
+    _apart((y,), (u, delta, z, Bm, Cm))
+    lib = capi.load()
+    if kept_states is not None:
+        _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
+    nbytes = lib.slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(dev, "slamhip_selective_scan_fwd", *ptrs, _strides(u, delta, z, Bm, Cm, y), _flat(A, F32, (C, N), dev, "A"),
+            _opt(D, F32, (C,), dev, "D"), _opt(delta_bias, F32, (C,), dev, "delta_bias"), _opt(state_in, F32, (B, C, N), dev, "state_in"),
+            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt],
+            _seq(y, dt, (B, T, C), dev, "y", out=True), _opt(state_out, F32, (B, C, N), dev, "state_out"), capi.ptr(kept_states),
+            capi.ptr(ws), nbytes)
+
+
+def selective_scan_bwd(dy, u, delta, A, Bm, Cm, kept_states, du, ddelta, dA, dB, dC, D=None, z=None, delta_bias=None, softplus=True,
+                       dD=None, dz=None, d_delta_bias=None, d_state_in=None, d_state_out=None, lengths=None):
+    """Gradients of selective_scan_fwd at the same inputs, with the states that it kept, from dy and from d_state_out, the
+    gradient that arrives at state_out: du, ddelta, dz (given when z is), dB, dC, dA, dD, d_delta_bias and d_state_in."""
+    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z)
+    outs = tuple(None if t is None else _seq(t, dt, (B, T, w), dev, what, out=True) for t, w, what in
+                 ((du, C, "du"), (ddelta, C, "ddelta"), (dz, C, "dz"), (dB, N, "dB"), (dC, N, "dC")))
+    if (z is None) != (dz is None) or du is None or ddelta is None or dB is None or dC is None:
+        raise ValueError("selective_scan_bwd: du, ddelta, dB, dC are wanted, and dz exactly when there is z")
+    _apart((du, ddelta, dz, dB, dC, d_state_in), (dy, u, delta, z, Bm, Cm, d_state_out))
+    lib = capi.load()
+    _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
+    nbytes = lib.slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "slamhip_selective_scan_bwd", _seq(dy, dt, (B, T, C), dev, "dy"), *ptrs,
+            _strides(dy, u, delta, z, Bm, Cm, du, ddelta, dz, dB, dC), _flat(A, F32, (C, N), dev, "A"), _opt(D, F32, (C,), dev, "D"),
+            _opt(delta_bias, F32, (C,), dev, "delta_bias"), kept_states.data_ptr(), _opt(d_state_out, F32, (B, C, N), dev, "d_state_out"),
+            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt], *outs,
+            _flat(dA, F32, (C, N), dev, "dA"), _opt(dD, F32, (C,), dev, "dD"), _opt(d_delta_bias, F32, (C,), dev, "d_delta_bias"),
+            _opt(d_state_in, F32, (B, C, N), dev, "d_state_in"), ws.data_ptr(), nbytes)

@@ -104,26 +104,36 @@ __device__ __forceinline__ void store_states(float* p, int N, int q, const float
     if (q * P + i < N) p[q * P + i] = v[i];
 }
 
-// B and C of steps [t0, t0 + TB) in float32, zeros beyond the sequence's end and beyond N
+// B and C of a block of steps, one value a thread and pass.  Loads are never guarded (a guarded load is waited for before the
+// next): rows that do not exist are read from a row that does, and what is not wanted is replaced by zero when it is stored.
 template <typename T, int P, int TB>
 struct Staged {
   static constexpr int kPer = TB * 8 * P / 256 > 0 ? TB * 8 * P / 256 : 1;
-  float v[kPer];
-  __device__ __forceinline__ void load(const ScanArgs& a, const Lane& l, int t0) {
+  const T* p[kPer];   // of the block that begins at step 0
+  long long st;
+  bool there[kPer];
+  int row[kPer];
+  T v[kPer];
+  __device__ __forceinline__ Staged(const ScanArgs& a, const Lane& l) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = i * 256 + threadIdx.x, n = at % (4 * P), which = at / (4 * P) & 1, t = t0 + at / (8 * P);
-      v[i] = 0.0f;
-      if (at < TB * 8 * P && n < a.N && t < l.len) {
-        const T* p = which ? (const T*)a.Cm + l.b * a.Cb + t * a.Ct : (const T*)a.Bm + l.b * a.Bb + t * a.Bt;
-        v[i] = (float)p[n];
-      }
+      const int at = (i * 256 + threadIdx.x) % (TB * 8 * P), n = at % (4 * P), which = at / (4 * P) & 1;
+      st = which ? a.Ct : a.Bt;
+      p[i] = (which ? (const T*)a.Cm + l.b * a.Cb : (const T*)a.Bm + l.b * a.Bb) + min(n, a.N - 1);
+      row[i] = at / (8 * P);
+      there[i] = n < a.N;
     }
   }
-  __device__ __forceinline__ void put(float* sh) const {
+  __device__ __forceinline__ void load(int t0, int T_) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i * 256 + threadIdx.x < TB * 8 * P) sh[i * 256 + threadIdx.x] = v[i];
+    for (int i = 0; i < kPer; ++i) v[i] = p[i][min(t0 + row[i], T_ - 1) * st];
+  }
+  __device__ __forceinline__ void put(float* sh, int t0, int len) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float f = there[i] && t0 + row[i] < len ? (float)v[i] : 0.0f;
+      if (TB * 8 * P >= 256 || threadIdx.x < TB * 8 * P) sh[i * 256 + threadIdx.x] = f;
+    }
   }
 };
 
@@ -133,16 +143,23 @@ __device__ __forceinline__ void read_states(const float* sh, float (&v)[P]) {
   for (int i = 0; i < P; ++i) v[i] = sh[i];
 }
 
-// a lane's own steps of a block: t0 + q, t0 + q + 4, ...; zero outside the sequence
+// a lane's own steps of a block: t0 + q, t0 + q + 4, ...; steps behind the tensor's end are read from its last row
 template <typename T, int G>
-__device__ __forceinline__ void load_own(const void* base, long long sb, long long st, const Lane& l, int t0, float (&v)[G]) {
-  const T* p = (const T*)base + l.b * sb + l.cc;
+struct Rows {
+  T* p;   // row q
+  long long st;
+  __device__ __forceinline__ Rows(const void* base, long long sb, long long st_, const Lane& l) : p((T*)base + l.b * sb + l.q * st_ + l.cc), st(st_) {}
+  __device__ __forceinline__ void load(T (&v)[G], int t0, int T_, int q) const {
+    if (t0 + 4 * G <= T_) {
 #pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const int t = t0 + 4 * i + l.q;
-    v[i] = t < l.own ? (float)p[t * st] : 0.0f;
+      for (int i = 0; i < G; ++i) v[i] = p[(t0 + 4 * i) * st];
+    } else {
+#pragma unroll
+      for (int i = 0; i < G; ++i) v[i] = p[(min(t0 + 4 * i + q, T_ - 1) - q) * st];
+    }
   }
-}
+  __device__ __forceinline__ void store(int t, float v) const { p[t * st] = (T)v; }   // row t + q
+};
 
 // STATES: the first pass of a cut sequence: each chunk's end state from zero (the first chunk's from state_in) and its sum of dt
 template <typename T, int P, bool STATES>
@@ -178,31 +195,33 @@ __global__ void __launch_bounds__(256) selective_scan_fwd_kernel(ScanArgs a) {
   const long long nblocks = (a.T + TB - 1) / TB;
   float dt_sum = 0.0f;
 
-  Staged<T, P, TB> next_bc;
-  float nu[G], nd[G], nz[G];
+  Staged<T, P, TB> next_bc(a, l);
+  const Rows<T, G> ru(a.u, a.ub, a.ut, l), rd(a.delta, a.deltab, a.deltat, l), rz(a.z, a.zb, a.zt, l), ry(a.y, a.yb, a.yt, l);
+  T nu[G], nd[G], nz[G];
   auto fetch = [&](int t0) {
-    next_bc.load(a, l, t0);
-    load_own<T, G>(a.u, a.ub, a.ut, l, t0, nu);
-    load_own<T, G>(a.delta, a.deltab, a.deltat, l, t0, nd);
-    if (!STATES && a.z) load_own<T, G>(a.z, a.zb, a.zt, l, t0, nz);
+    next_bc.load(t0, a.T);
+    ru.load(nu, t0, a.T, l.q);
+    rd.load(nd, t0, a.T, l.q);
+    if (!STATES && a.z) rz.load(nz, t0, a.T, l.q);
   };
   if (t_begin < t_end) fetch(t_begin);
   int buf = 0;
   for (int t0 = t_begin; t0 < t_end; t0 += TB, buf ^= 1) {
     if (!STATES && a.kept && l.live)
       store_states<P>(a.kept + (((long long)l.b * nblocks + t0 / TB) * a.C + l.c) * a.N, a.N, l.q, h);
-    next_bc.put(bc[buf]);
+    next_bc.put(bc[buf], t0, l.len);
     float u[G], dt[G], x[G], z[G];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const float raw = nd[i] + bias;
+      const bool in = t0 + 4 * i + l.q < l.own;
+      const float raw = (float)nd[i] + bias;
       dt[i] = raw;
       if (a.softplus) dt[i] = softplus_(raw, exp2_(-kLog2e * fabsf(raw)));
-      if (t0 + 4 * i + l.q >= l.own) dt[i] = 0.0f;
-      u[i] = nu[i];
+      if (!in) dt[i] = 0.0f;
+      u[i] = in ? (float)nu[i] : 0.0f;
       x[i] = dt[i] * u[i];
       dt_sum += dt[i];
-      if (!STATES && a.z) z[i] = nz[i];
+      if (!STATES && a.z) z[i] = (float)nz[i];
     }
     __syncthreads();   // bc[buf] is whole; bc[buf ^ 1] has been read by all
     if (t0 + TB < t_end) fetch(t0 + TB);
@@ -233,7 +252,7 @@ __global__ void __launch_bounds__(256) selective_scan_fwd_kernel(ScanArgs a) {
         float v = fmaf(D, u[i], quad_sum_own(inner, l.q));
         if (a.z) v *= z[i] * sigmoid_(z[i]);
         if (t >= l.len) v = 0.0f;
-        if (l.live && t < t_end) ((T*)a.y + l.b * a.yb + t * a.yt)[l.c] = (T)v;
+        if (l.live && t < t_end) ry.store(t0 + 4 * i, v);
       }
     }
   }
@@ -320,36 +339,49 @@ __global__ void __launch_bounds__(256, 2) selective_scan_bwd_kernel(ScanArgs a) 
   const int groups = gridDim.x;
   float dt_sum = 0.0f, dD = 0.0f, dbias = 0.0f;
 
-  for (int t0 = t_begin + (t_end - 1 - t_begin) / TB * TB; t0 >= t_begin && t_begin < t_end; t0 -= TB) {
-    Staged<T, P, TB> stage;
-    stage.load(a, l, t0);
-    float u[G], raw[G], z[G], dy[G], dt[G], e[G], slope[G];
-    load_own<T, G>(a.u, a.ub, a.ut, l, t0, u);
-    load_own<T, G>(a.delta, a.deltab, a.deltat, l, t0, raw);
-    load_own<T, G>(a.dy, a.dyb, a.dyt, l, t0, dy);
-    if (a.z) load_own<T, G>(a.z, a.zb, a.zt, l, t0, z);
-    float h[P];
-    if (!CARRY) load_states<P>(a.kept + (((long long)l.b * nblocks + t0 / TB) * a.C + l.cc) * a.N, a.N, l.q, h);
+  Staged<T, P, TB> next_bc(a, l);
+  const Rows<T, G> ru(a.u, a.ub, a.ut, l), rd(a.delta, a.deltab, a.deltat, l), rz(a.z, a.zb, a.zt, l), ry(a.dy, a.dyb, a.dyt, l);
+  const Rows<T, G> rdu(a.du, a.dub, a.dut, l), rdd(a.ddelta, a.ddeltab, a.ddeltat, l), rdz(a.dz, a.dzb, a.dzt, l);
+  const float* kept = a.kept + ((long long)l.b * nblocks * a.C + l.cc) * a.N;
+  T nu[G], nd[G], nz[G], ny[G];
+  float h[P];
+  auto fetch = [&](int t0) {
+    next_bc.load(t0, a.T);
+    if (!CARRY) ru.load(nu, t0, a.T, l.q);
+    rd.load(nd, t0, a.T, l.q);
+    ry.load(ny, t0, a.T, l.q);
+    if (a.z) rz.load(nz, t0, a.T, l.q);
+  };
+  const int t_last = t_begin + (t_end - 1 - t_begin) / TB * TB;
+  if (t_begin < t_end) fetch(t_last);
+  for (int t0 = t_last; t0 >= t_begin && t_begin < t_end; t0 -= TB) {
+    if (!CARRY) load_states<P>(kept + (long long)(t0 / TB) * a.C * a.N, a.N, l.q, h);
+    float u[G], z[G], dy[G], dt[G], e[G], slope[G];
     __syncthreads();   // the previous block's bc and bc_grad have been read
-    stage.put(bc);
+    next_bc.put(bc, t0, l.len);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const bool in = t0 + 4 * i + l.q < l.own;
-      const float r = raw[i] + bias;
+      const float r = (float)nd[i] + bias;
       dt[i] = r;
       slope[i] = 1.0f;
       if (a.softplus) {
         const float x = exp2_(-kLog2e * fabsf(r));
         dt[i] = softplus_(r, x);
-        slope[i] = (r >= 0.0f ? 1.0f : x) * rcp_(1.0f + x);
+        if (!CARRY) slope[i] = (r >= 0.0f ? 1.0f : x) * rcp_(1.0f + x);
       }
       if (!in) dt[i] = 0.0f;
-      e[i] = dy[i];
-      if (a.z) e[i] *= z[i] * sigmoid_(z[i]);
+      if (!CARRY) u[i] = in ? (float)nu[i] : 0.0f;
+      e[i] = dy[i] = (float)ny[i];
+      if (a.z) {
+        z[i] = (float)nz[i];
+        e[i] *= z[i] * sigmoid_(z[i]);
+      }
       if (!in) e[i] = 0.0f;
       dt_sum += dt[i];
     }
     __syncthreads();
+    if (t0 - TB >= t_begin) fetch(t0 - TB);
     if (CARRY) {
 #pragma unroll
       for (int i = G - 1; i >= 0; --i) {
@@ -444,13 +476,13 @@ __global__ void __launch_bounds__(256, 2) selective_scan_bwd_kernel(ScanArgs a) 
       dD = fmaf(e[i], u[i], dD);
       dbias += dd;
       if (l.live && t < t_end) {
-        ((T*)a.du + l.b * a.dub + t * a.dut)[l.c] = (T)du;
-        ((T*)a.ddelta + l.b * a.ddeltab + t * a.ddeltat)[l.c] = (T)dd;
+        rdu.store(t0 + 4 * i, du);
+        rdd.store(t0 + 4 * i, dd);
         if (a.dz) {
           const float s = sigmoid_(z[i]);
           float dz = dy[i] * fmaf(D, u[i], in_sum) * s * fmaf(z[i], 1.0f - s, 1.0f);
           if (!in) dz = 0.0f;
-          ((T*)a.dz + l.b * a.dzb + t * a.dzt)[l.c] = (T)dz;
+          rdz.store(t0 + 4 * i, dz);
         }
       }
     }

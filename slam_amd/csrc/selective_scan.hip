@@ -25,9 +25,14 @@
 namespace slamhip {
 namespace {
 
-// steps that the states are kept apart: the backward pass holds TB * P states and as many decays a lane
-constexpr int block_steps(int P) { return P == 8 ? 8 : 16; }
+// steps that the states are kept apart, and that the backward pass works on at once: it holds as many states and decays of each
+// of a lane's P in registers
+constexpr int kept_steps(int P) { return P <= 2 ? 16 : 8; }
+constexpr int kFwdSteps = 16;   // steps that the forward pass stages at once
 
+#ifndef BWD_OCC
+#define BWD_OCC 2
+#endif
 struct ScanArgs {
   const void *u, *delta, *z, *Bm, *Cm, *dy;
   const float *A, *D, *bias, *state_in, *d_state_out;
@@ -72,7 +77,7 @@ __device__ __forceinline__ float softplus_(float v, float e) {
 
 struct Lane {
   int q, c, cc, len, own, b;   // own: the lane's own length, 0 without a channel
-  bool live;
+  bool live, whole;            // whole: all channels of the workgroup are there
 };
 
 __device__ __forceinline__ Lane scan_lane(const ScanArgs& a) {
@@ -88,52 +93,74 @@ __device__ __forceinline__ Lane scan_lane(const ScanArgs& a) {
     l.len = n < 0 ? 0 : (n > a.T ? a.T : n);
   }
   l.own = l.live ? l.len : 0;
+  l.whole = (blockIdx.x + 1) * 64 <= (unsigned)a.C;
   return l;
 }
 
+// a lane's P states of a row of N; all lanes' are there when N == 4 P
+template <int P>
+struct StateVector {
+  typedef float type __attribute__((ext_vector_type(P), aligned(4)));
+};
+template <>
+struct StateVector<1> {
+  typedef float type;
+};
+
 template <int P>
 __device__ __forceinline__ void load_states(const float* p, int N, int q, float (&v)[P]) {
+  if (P > 1 && N == 4 * P) {
+    const typename StateVector<P>::type r = *reinterpret_cast<const typename StateVector<P>::type*>(p + q * P);
+    __builtin_memcpy(v, &r, sizeof(v));
+  } else {
 #pragma unroll
-  for (int i = 0; i < P; ++i) v[i] = q * P + i < N ? p[q * P + i] : 0.0f;
+    for (int i = 0; i < P; ++i) v[i] = q * P + i < N ? p[q * P + i] : 0.0f;
+  }
 }
 
 template <int P>
 __device__ __forceinline__ void store_states(float* p, int N, int q, const float (&v)[P]) {
+  if (P > 1 && N == 4 * P) {
+    typename StateVector<P>::type r;
+    __builtin_memcpy(&r, v, sizeof(v));
+    *reinterpret_cast<typename StateVector<P>::type*>(p + q * P) = r;
+  } else {
 #pragma unroll
-  for (int i = 0; i < P; ++i)
-    if (q * P + i < N) p[q * P + i] = v[i];
+    for (int i = 0; i < P; ++i)
+      if (q * P + i < N) p[q * P + i] = v[i];
+  }
 }
 
-// B and C of a block of steps, one value a thread and pass.  Loads are never guarded (a guarded load is waited for before the
-// next): rows that do not exist are read from a row that does, and what is not wanted is replaced by zero when it is stored.
+// B and C of a block of steps, one value a thread and pass; zeros beyond the sequence's end and beyond N.  The values stay in the
+// sequences' type until they are put away: a conversion behind a guarded load would be waited for before the next load.
 template <typename T, int P, int TB>
 struct Staged {
   static constexpr int kPer = TB * 8 * P / 256 > 0 ? TB * 8 * P / 256 : 1;
-  const T* p[kPer];   // of the block that begins at step 0
+  const T* p;           // value 0 of the thread; the next ones are `rows` steps on
   long long st;
-  bool there[kPer];
-  int row[kPer];
+  bool there;
+  int row;
   T v[kPer];
-  __device__ __forceinline__ Staged(const ScanArgs& a, const Lane& l) {
+  __device__ __forceinline__ Staged(const ScanArgs& a, const Lane& l, int t0) {
+    const int at = threadIdx.x % (TB * 8 * P), n = at % (4 * P), which = at / (4 * P) & 1;
+    st = which ? a.Ct : a.Bt;
+    row = at / (8 * P);
+    p = (which ? (const T*)a.Cm + l.b * a.Cb : (const T*)a.Bm + l.b * a.Bb) + n + (long long)(t0 + row) * st;
+    there = n < a.N;
+  }
+  static constexpr int kRows = 256 / (8 * P);
+  __device__ __forceinline__ void load(int t0, int len) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = (i * 256 + threadIdx.x) % (TB * 8 * P), n = at % (4 * P), which = at / (4 * P) & 1;
-      st = which ? a.Ct : a.Bt;
-      p[i] = (which ? (const T*)a.Cm + l.b * a.Cb : (const T*)a.Bm + l.b * a.Bb) + min(n, a.N - 1);
-      row[i] = at / (8 * P);
-      there[i] = n < a.N;
+      v[i] = (T)0.0f;
+      if (there && t0 + row + i * kRows < len) v[i] = p[i * kRows * st];
     }
   }
-  __device__ __forceinline__ void load(int t0, int T_) {
+  __device__ __forceinline__ void advance(int steps) { p += steps * st; }
+  __device__ __forceinline__ void put(float* sh) const {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = p[i][min(t0 + row[i], T_ - 1) * st];
-  }
-  __device__ __forceinline__ void put(float* sh, int t0, int len) const {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const float f = there[i] && t0 + row[i] < len ? (float)v[i] : 0.0f;
-      if (TB * 8 * P >= 256 || threadIdx.x < TB * 8 * P) sh[i * 256 + threadIdx.x] = f;
-    }
+    for (int i = 0; i < kPer; ++i)
+      if (TB * 8 * P >= 256 || threadIdx.x < TB * 8 * P) sh[i * 256 + threadIdx.x] = (float)v[i];
   }
 };
 
@@ -143,28 +170,34 @@ __device__ __forceinline__ void read_states(const float* sh, float (&v)[P]) {
   for (int i = 0; i < P; ++i) v[i] = sh[i];
 }
 
-// a lane's own steps of a block: t0 + q, t0 + q + 4, ...; steps behind the tensor's end are read from its last row
+// a lane's own steps of a block: t0 + q, t0 + q + 4, ...; the pointer moves with the block (a product of 64 bits for every access
+// costs as much as the recurrence)
 template <typename T, int G>
 struct Rows {
-  T* p;   // row q
-  long long st;
-  __device__ __forceinline__ Rows(const void* base, long long sb, long long st_, const Lane& l) : p((T*)base + l.b * sb + l.q * st_ + l.cc), st(st_) {}
-  __device__ __forceinline__ void load(T (&v)[G], int t0, int T_, int q) const {
-    if (t0 + 4 * G <= T_) {
+  T* p;             // step t0 + q
+  long long four;   // four steps
+  __device__ __forceinline__ Rows(const void* base, long long sb, long long st, const Lane& l, int t0)
+      : p((T*)base + l.b * sb + (t0 + l.q) * st + l.cc), four(4 * st) {}
+  __device__ __forceinline__ void load(T (&v)[G], bool full, int t0, const Lane& l) const {
+    if (full) {
 #pragma unroll
-      for (int i = 0; i < G; ++i) v[i] = p[(t0 + 4 * i) * st];
+      for (int i = 0; i < G; ++i) v[i] = p[i * four];
     } else {
 #pragma unroll
-      for (int i = 0; i < G; ++i) v[i] = p[(min(t0 + 4 * i + q, T_ - 1) - q) * st];
+      for (int i = 0; i < G; ++i) {
+        v[i] = (T)0.0f;
+        if (t0 + 4 * i + l.q < l.own) v[i] = p[i * four];
+      }
     }
   }
-  __device__ __forceinline__ void store(int t, float v) const { p[t * st] = (T)v; }   // row t + q
+  __device__ __forceinline__ void store(int i, float v) const { p[i * four] = (T)v; }
+  __device__ __forceinline__ void advance(int fours) { p += fours * four; }
 };
 
 // STATES: the first pass of a cut sequence: each chunk's end state from zero (the first chunk's from state_in) and its sum of dt
 template <typename T, int P, bool STATES>
 __global__ void __launch_bounds__(256) selective_scan_fwd_kernel(ScanArgs a) {
-  constexpr int TB = block_steps(P), G = TB / 4;
+  constexpr int TB = kFwdSteps, G = TB / 4, TK = kept_steps(P);
   __shared__ float bc[2][TB * 8 * P];
   const Lane l = scan_lane(a);
   const int chunk = blockIdx.y, t_begin = chunk * a.chunk, t_end = min(t_begin + a.chunk, a.T);
@@ -192,41 +225,52 @@ __global__ void __launch_bounds__(256) selective_scan_fwd_kernel(ScanArgs a) {
     }
   }
   const float bias = a.bias ? a.bias[l.cc] : 0.0f, D = a.D ? a.D[l.cc] : 0.0f;
-  const long long nblocks = (a.T + TB - 1) / TB;
+  const long long nkept = (a.T + TK - 1) / TK;
   float dt_sum = 0.0f;
 
-  Staged<T, P, TB> next_bc(a, l);
-  const Rows<T, G> ru(a.u, a.ub, a.ut, l), rd(a.delta, a.deltab, a.deltat, l), rz(a.z, a.zb, a.zt, l), ry(a.y, a.yb, a.yt, l);
+  Staged<T, P, TB> next_bc(a, l, t_begin);
+  Rows<T, G> ru(a.u, a.ub, a.ut, l, t_begin), rd(a.delta, a.deltab, a.deltat, l, t_begin), rz(a.z, a.zb, a.zt, l, t_begin);
+  Rows<T, G> ry(a.y, a.yb, a.yt, l, t_begin);
+  float* kept = a.kept + (((long long)l.b * nkept + t_begin / TK) * a.C + l.c) * a.N;
+  const long long kept_step = (long long)a.C * a.N;
   T nu[G], nd[G], nz[G];
   auto fetch = [&](int t0) {
-    next_bc.load(t0, a.T);
-    ru.load(nu, t0, a.T, l.q);
-    rd.load(nd, t0, a.T, l.q);
-    if (!STATES && a.z) rz.load(nz, t0, a.T, l.q);
+    const bool full = l.whole && t0 + TB <= l.len;
+    next_bc.load(t0, l.len);
+    ru.load(nu, full, t0, l);
+    rd.load(nd, full, t0, l);
+    if (!STATES && a.z) rz.load(nz, full, t0, l);
+    next_bc.advance(TB);
+    ru.advance(G);
+    rd.advance(G);
+    if (!STATES) rz.advance(G);
   };
   if (t_begin < t_end) fetch(t_begin);
   int buf = 0;
   for (int t0 = t_begin; t0 < t_end; t0 += TB, buf ^= 1) {
-    if (!STATES && a.kept && l.live)
-      store_states<P>(a.kept + (((long long)l.b * nblocks + t0 / TB) * a.C + l.c) * a.N, a.N, l.q, h);
-    next_bc.put(bc[buf], t0, l.len);
+    next_bc.put(bc[buf]);
     float u[G], dt[G], x[G], z[G];
 #pragma unroll
+    for (int i = 0; i < G; ++i) dt[i] = (float)nd[i] + bias;
+    if (a.softplus)
+#pragma unroll
+      for (int i = 0; i < G; ++i) dt[i] = softplus_(dt[i], exp2_(-kLog2e * fabsf(dt[i])));
+#pragma unroll
     for (int i = 0; i < G; ++i) {
-      const bool in = t0 + 4 * i + l.q < l.own;
-      const float raw = (float)nd[i] + bias;
-      dt[i] = raw;
-      if (a.softplus) dt[i] = softplus_(raw, exp2_(-kLog2e * fabsf(raw)));
-      if (!in) dt[i] = 0.0f;
-      u[i] = in ? (float)nu[i] : 0.0f;
+      if (t0 + 4 * i + l.q >= l.own) dt[i] = 0.0f;
+      u[i] = (float)nu[i];
       x[i] = dt[i] * u[i];
-      dt_sum += dt[i];
+      if (STATES) dt_sum += dt[i];
       if (!STATES && a.z) z[i] = (float)nz[i];
     }
     __syncthreads();   // bc[buf] is whole; bc[buf ^ 1] has been read by all
     if (t0 + TB < t_end) fetch(t0 + TB);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
+      if (!STATES && i % (TK / 4) == 0 && a.kept) {
+        if (l.live && t0 + 4 * i < a.T) store_states<P>(kept, a.N, l.q, h);
+        kept += kept_step;
+      }
       float inner[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       if (t0 + 4 * i < l.len) {
         auto step = [&](auto k) {
@@ -252,9 +296,10 @@ __global__ void __launch_bounds__(256) selective_scan_fwd_kernel(ScanArgs a) {
         float v = fmaf(D, u[i], quad_sum_own(inner, l.q));
         if (a.z) v *= z[i] * sigmoid_(z[i]);
         if (t >= l.len) v = 0.0f;
-        if (l.live && t < t_end) ry.store(t0 + 4 * i, v);
+        if (l.live && t < t_end) ry.store(i, v);
       }
     }
+    if (!STATES) ry.advance(G);
   }
   if (STATES) {
     if (l.live) {
@@ -308,10 +353,10 @@ __device__ __forceinline__ int channel_sum_index(int i, int row) {
 
 // CARRY: the first pass of a cut sequence: the gradient that each chunk by itself hands to the state in front of it
 template <typename T, int P, bool CARRY>
-__global__ void __launch_bounds__(256, 2) selective_scan_bwd_kernel(ScanArgs a) {
-  constexpr int TB = block_steps(P), G = TB / 4;
-  __shared__ float bc[TB * 8 * P];
-  __shared__ float bc_grad[CARRY ? 1 : 4][CARRY ? 1 : TB * 8 * P];
+__global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : BWD_OCC) selective_scan_bwd_kernel(ScanArgs a) {
+  constexpr int TB = kept_steps(P), G = TB / 4, V = TB * 8 * P;
+  __shared__ float bc[2][V];
+  __shared__ float bc_grad[CARRY ? 1 : 2][CARRY ? 1 : 4][CARRY ? 1 : V];
   const Lane l = scan_lane(a);
   const int wave = threadIdx.x >> 6;
   const int chunk = blockIdx.y, t_begin = chunk * a.chunk, t_end = min(t_begin + a.chunk, a.T);
@@ -335,59 +380,84 @@ __global__ void __launch_bounds__(256, 2) selective_scan_bwd_kernel(ScanArgs a) 
       for (int i = 0; i < P; ++i) g[i] = j == a.chunks - 1 ? e[i] : fmaf(exp2_(A2[i] * s), g[i], e[i]);
     }
   const float bias = a.bias ? a.bias[l.cc] : 0.0f, D = a.D ? a.D[l.cc] : 0.0f;
-  const long long nblocks = (a.T + TB - 1) / TB;
+  const long long nkept = (a.T + TB - 1) / TB;
   const int groups = gridDim.x;
   float dt_sum = 0.0f, dD = 0.0f, dbias = 0.0f;
 
-  Staged<T, P, TB> next_bc(a, l);
-  const Rows<T, G> ru(a.u, a.ub, a.ut, l), rd(a.delta, a.deltab, a.deltat, l), rz(a.z, a.zb, a.zt, l), ry(a.dy, a.dyb, a.dyt, l);
-  const Rows<T, G> rdu(a.du, a.dub, a.dut, l), rdd(a.ddelta, a.ddeltab, a.ddeltat, l), rdz(a.dz, a.dzb, a.dzt, l);
-  const float* kept = a.kept + ((long long)l.b * nblocks * a.C + l.cc) * a.N;
-  T nu[G], nd[G], nz[G], ny[G];
-  float h[P];
-  auto fetch = [&](int t0) {
-    next_bc.load(t0, a.T);
-    if (!CARRY) ru.load(nu, t0, a.T, l.q);
-    rd.load(nd, t0, a.T, l.q);
-    ry.load(ny, t0, a.T, l.q);
-    if (a.z) rz.load(nz, t0, a.T, l.q);
-  };
   const int t_last = t_begin + (t_end - 1 - t_begin) / TB * TB;
-  if (t_begin < t_end) fetch(t_last);
-  for (int t0 = t_last; t0 >= t_begin && t_begin < t_end; t0 -= TB) {
-    if (!CARRY) load_states<P>(kept + (long long)(t0 / TB) * a.C * a.N, a.N, l.q, h);
-    float u[G], z[G], dy[G], dt[G], e[G], slope[G];
-    __syncthreads();   // the previous block's bc and bc_grad have been read
-    next_bc.put(bc, t0, l.len);
+  Staged<T, P, TB> next_bc(a, l, t_last);
+  Rows<T, G> ru(a.u, a.ub, a.ut, l, t_last), rd(a.delta, a.deltab, a.deltat, l, t_last), rz(a.z, a.zb, a.zt, l, t_last);
+  Rows<T, G> ry(a.dy, a.dyb, a.dyt, l, t_last), rdu(a.du, a.dub, a.dut, l, t_last), rdd(a.ddelta, a.ddeltab, a.ddeltat, l, t_last);
+  Rows<T, G> rdz(a.dz, a.dzb, a.dzt, l, t_last);
+  const float* kept = a.kept + (((long long)l.b * nkept + t_last / TB) * a.C + l.cc) * a.N;
+  T nu[G], nd[G], nz[G], ny[G];
+  float nh[P];
+  auto fetch = [&](int t0) {
+    const bool full = l.whole && t0 + TB <= l.len;
+    next_bc.load(t0, l.len);
+    if (!CARRY) {
+      load_states<P>(kept, a.N, l.q, nh);
+      kept -= (long long)a.C * a.N;
+      ru.load(nu, full, t0, l);
+      ru.advance(-G);
+    }
+    rd.load(nd, full, t0, l);
+    ry.load(ny, full, t0, l);
+    if (a.z) rz.load(nz, full, t0, l);
+    next_bc.advance(-TB);
+    rd.advance(-G);
+    ry.advance(-G);
+    rz.advance(-G);
+  };
+  // part_bc [B][T][groups][2][4 P]: a block's dB and dC of the workgroup's channels, once all waves have left theirs
+  float* part_bc = a.part_bc + (((long long)l.b * a.T + t_last + threadIdx.x / (8 * P)) * groups + blockIdx.x) * 8 * P + threadIdx.x % (8 * P);
+  const long long part_row = (long long)groups * 8 * P;
+  auto put_part = [&](int t0, int buf) {
+    if constexpr (!CARRY) {
+      constexpr int kRows = 256 / (8 * P);
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const bool in = t0 + 4 * i + l.q < l.own;
-      const float r = (float)nd[i] + bias;
-      dt[i] = r;
-      slope[i] = 1.0f;
-      if (a.softplus) {
-        const float x = exp2_(-kLog2e * fabsf(r));
-        dt[i] = softplus_(r, x);
-        if (!CARRY) slope[i] = (r >= 0.0f ? 1.0f : x) * rcp_(1.0f + x);
+      for (int i = 0; i < (V + 255) / 256; ++i) {
+        const int at = i * 256 + threadIdx.x;
+        if (at < V && t0 + at / (8 * P) < t_end)
+          part_bc[i * kRows * part_row] = (bc_grad[buf][0][at] + bc_grad[buf][1][at]) + (bc_grad[buf][2][at] + bc_grad[buf][3][at]);
       }
-      if (!in) dt[i] = 0.0f;
-      if (!CARRY) u[i] = in ? (float)nu[i] : 0.0f;
+      part_bc -= TB * part_row;
+    }
+  };
+  int buf = 0;
+  if (t_begin < t_end) fetch(t_last);
+  for (int t0 = t_last; t0 >= t_begin && t_begin < t_end; t0 -= TB, buf ^= 1) {
+    float u[G], z[G], dy[G], raw[G], dt[G], e[G], h[P];
+    next_bc.put(bc[buf]);
+#pragma unroll
+    for (int i = 0; i < G; ++i) dt[i] = raw[i] = (float)nd[i] + bias;
+    if (a.softplus)
+#pragma unroll
+      for (int i = 0; i < G; ++i) dt[i] = softplus_(raw[i], exp2_(-kLog2e * fabsf(raw[i])));
+#pragma unroll
+    for (int i = 0; i < G; ++i) {   // behind the sequence u, dy and z are zero
+      if (t0 + 4 * i + l.q >= l.own) dt[i] = 0.0f;
+      if (!CARRY) u[i] = (float)nu[i];
       e[i] = dy[i] = (float)ny[i];
-      if (a.z) {
+      if (CARRY) dt_sum += dt[i];
+    }
+    if (a.z)
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
         z[i] = (float)nz[i];
         e[i] *= z[i] * sigmoid_(z[i]);
       }
-      if (!in) e[i] = 0.0f;
-      dt_sum += dt[i];
-    }
-    __syncthreads();
+    if (!CARRY)
+#pragma unroll
+      for (int i = 0; i < P; ++i) h[i] = nh[i];
+    __syncthreads();   // bc[buf] is whole, and so is the previous block's bc_grad; what was read two blocks ago may be written
     if (t0 - TB >= t_begin) fetch(t0 - TB);
-    if (CARRY) {
+    if constexpr (CARRY) {
 #pragma unroll
       for (int i = G - 1; i >= 0; --i) {
         auto step = [&](auto k) {
           constexpr int K = decltype(k)::value;
-          const float* sh = bc + (4 * i + K) * 8 * P + l.q * P;
+          const float* sh = bc[buf] + (4 * i + K) * 8 * P + l.q * P;
           float Cv[P];
           read_states<P>(sh + 4 * P, Cv);
           const float d = quad_lane<K>(dt[i]), ev = quad_lane<K>(e[i]);
@@ -399,120 +469,120 @@ __global__ void __launch_bounds__(256, 2) selective_scan_bwd_kernel(ScanArgs a) 
         step(std::integral_constant<int, 1>{});
         step(std::integral_constant<int, 0>{});
       }
-      continue;
-    }
-    float hs[TB][P], as[TB][P];   // the state in front of each step, and its decay
+    } else {
+      if (t0 + TB < t_end) put_part(t0 + TB, buf ^ 1);
+      float hs[TB][P], as[TB][P];   // the state in front of each step, and its decay
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const float x = dt[i] * u[i];
-      auto step = [&](auto k) {
-        constexpr int K = decltype(k)::value;
-        const float* sh = bc + (4 * i + K) * 8 * P + l.q * P;
-        float Bv[P];
-        read_states<P>(sh, Bv);
-        const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x);
+      for (int i = 0; i < G; ++i) {
+        const float x = dt[i] * u[i];
+        auto step = [&](auto k) {
+          constexpr int K = decltype(k)::value;
+          const float* sh = bc[buf] + (4 * i + K) * 8 * P + l.q * P;
+          float Bv[P];
+          read_states<P>(sh, Bv);
+          const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x);
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          hs[4 * i + K][p] = h[p];
-          as[4 * i + K][p] = exp2_(A2[p] * d);
-          h[p] = fmaf(as[4 * i + K][p], h[p], xv * Bv[p]);
-        }
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-      step(std::integral_constant<int, 2>{});
-      step(std::integral_constant<int, 3>{});
-    }
+          for (int p = 0; p < P; ++p) {
+            hs[4 * i + K][p] = h[p];
+            as[4 * i + K][p] = exp2_(A2[p] * d);
+            h[p] = fmaf(as[4 * i + K][p], h[p], xv * Bv[p]);
+          }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+      }
 #pragma unroll
-    for (int i = G - 1; i >= 0; --i) {
-      const float x = dt[i] * u[i];
-      float inner[4], gb[4], qa[4];
-      auto step = [&](auto k) {
-        constexpr int K = decltype(k)::value;
-        const float* sh = bc + (4 * i + K) * 8 * P + l.q * P;
-        float Bv[P], Cv[P], v[2 * P];
-        read_states<P>(sh, Bv);
-        read_states<P>(sh + 4 * P, Cv);
-        const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x), ev = quad_lane<K>(e[i]);
-        float s_in = 0.0f, s_gb = 0.0f, s_qa = 0.0f;
+      for (int i = G - 1; i >= 0; --i) {
+        const float x = dt[i] * u[i];
+        float inner[4], gb[4], qa[4];
+        auto step = [&](auto k) {
+          constexpr int K = decltype(k)::value;
+          const float* sh = bc[buf] + (4 * i + K) * 8 * P + l.q * P;
+          float Bv[P], Cv[P], v[2 * P];
+          read_states<P>(sh, Bv);
+          read_states<P>(sh + 4 * P, Cv);
+          const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x), ev = quad_lane<K>(e[i]);
+          float s_in = 0.0f, s_gb = 0.0f, s_qa = 0.0f;
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          g[p] = fmaf(ev, Cv[p], g[p]);
-          s_in = fmaf(h[p], Cv[p], s_in);
-          v[P + p] = ev * h[p];
-          v[p] = g[p] * xv;
-          s_gb = fmaf(g[p], Bv[p], s_gb);
-          g[p] *= as[4 * i + K][p];
-          h[p] = hs[4 * i + K][p];
-          const float q = g[p] * h[p];
-          dA[p] = fmaf(q, d, dA[p]);
-          s_qa = fmaf(q, A2[p], s_qa);
-        }
-        inner[K] = s_in;
-        gb[K] = s_gb;
-        qa[K] = s_qa;
-        channel_sums<P>(v);
-        constexpr int R = P >= 2 ? P / 2 : 1;
-        if ((threadIdx.x & 12) == 0) {   // the first channel of each row
-          const int row = threadIdx.x >> 4 & 3;
-          float* out = bc_grad[wave] + (4 * i + K) * 8 * P;
+          for (int p = 0; p < P; ++p) {
+            g[p] = fmaf(ev, Cv[p], g[p]);
+            s_in = fmaf(h[p], Cv[p], s_in);
+            v[P + p] = ev * h[p];
+            v[p] = g[p] * xv;
+            s_gb = fmaf(g[p], Bv[p], s_gb);
+            g[p] *= as[4 * i + K][p];
+            h[p] = hs[4 * i + K][p];
+            const float q = g[p] * h[p];
+            dA[p] = fmaf(q, d, dA[p]);
+            s_qa = fmaf(q, A2[p], s_qa);
+          }
+          inner[K] = s_in;
+          gb[K] = s_gb;
+          qa[K] = s_qa;
+          channel_sums<P>(v);
+          constexpr int R = P >= 2 ? P / 2 : 1;
+          if ((threadIdx.x & 12) == 0) {   // the first channel of each row
+            const int row = threadIdx.x >> 4 & 3;
+            float* out = bc_grad[buf][wave] + (4 * i + K) * 8 * P;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const int at = channel_sum_index<P>(r, row);   // below P: dB of state at, else dC of state at - P
-            out[(at >= P ? 4 * P + at - P : at) + l.q * P] = v[r];
+            for (int r = 0; r < R; ++r) {
+              const int at = channel_sum_index<P>(r, row);   // below P: dB of state at, else dC of state at - P
+              out[(at >= P ? 4 * P + at - P : at) + l.q * P] = v[r];
+            }
+          }
+        };
+        step(std::integral_constant<int, 3>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 0>{});
+        const int t = t0 + 4 * i + l.q;
+        const float in_sum = quad_sum_own(inner, l.q), gb_sum = quad_sum_own(gb, l.q), qa_sum = quad_sum_own(qa, l.q);
+        const bool in = t < l.own;
+        float slope = 1.0f;
+        if (a.softplus) slope = sigmoid_(raw[i]);
+        float du = fmaf(gb_sum, dt[i], D * e[i]);
+        float dd = fmaf(gb_sum, u[i], qa_sum * kLn2) * slope;
+        if (!in) du = dd = 0.0f;
+        dD = fmaf(e[i], u[i], dD);
+        dbias += dd;
+        if (l.live && t < t_end) {
+          rdu.store(i, du);
+          rdd.store(i, dd);
+          if (a.dz) {
+            const float s = sigmoid_(z[i]);
+            float dz = dy[i] * fmaf(D, u[i], in_sum) * s * fmaf(z[i], 1.0f - s, 1.0f);
+            if (!in) dz = 0.0f;
+            rdz.store(i, dz);
           }
         }
-      };
-      step(std::integral_constant<int, 3>{});
-      step(std::integral_constant<int, 2>{});
-      step(std::integral_constant<int, 1>{});
-      step(std::integral_constant<int, 0>{});
-      const int t = t0 + 4 * i + l.q;
-      const float in_sum = quad_sum_own(inner, l.q), gb_sum = quad_sum_own(gb, l.q), qa_sum = quad_sum_own(qa, l.q);
-      const bool in = t < l.len;
-      float du = fmaf(gb_sum, dt[i], D * e[i]);
-      float dd = fmaf(gb_sum, u[i], qa_sum * kLn2) * slope[i];
-      if (!in) du = dd = 0.0f;
-      dD = fmaf(e[i], u[i], dD);
-      dbias += dd;
-      if (l.live && t < t_end) {
-        rdu.store(t0 + 4 * i, du);
-        rdd.store(t0 + 4 * i, dd);
-        if (a.dz) {
-          const float s = sigmoid_(z[i]);
-          float dz = dy[i] * fmaf(D, u[i], in_sum) * s * fmaf(z[i], 1.0f - s, 1.0f);
-          if (!in) dz = 0.0f;
-          rdz.store(t0 + 4 * i, dz);
-        }
       }
-    }
-    __syncthreads();
-    // part_bc [B][T][groups][2][4 P]
-    for (int at = threadIdx.x; at < TB * 8 * P; at += 256) {
-      const int t = t0 + at / (8 * P);
-      if (t < t_end)
-        a.part_bc[(((long long)l.b * a.T + t) * groups + blockIdx.x) * 8 * P + at % (8 * P)] =
-            (bc_grad[0][at] + bc_grad[1][at]) + (bc_grad[2][at] + bc_grad[3][at]);
+      rdu.advance(-G);
+      rdd.advance(-G);
+      rdz.advance(-G);
     }
   }
-  if (CARRY) {
+  if constexpr (CARRY) {
     if (l.live) {
       store_states<P>(a.ends + (((long long)l.b * a.chunks + chunk) * a.C + l.c) * a.N, a.N, l.q, g);
       const float s = quad_sum(dt_sum);
       if (l.q == 0) a.sums[((long long)l.b * a.chunks + chunk) * a.C + l.c] = s;
     }
-    return;
-  }
-  dD = quad_sum(dD);
-  dbias = quad_sum(dbias);
-  if (l.live) {
-    if (a.d_state_in && chunk == 0) store_states<P>(a.d_state_in + bC * a.N, a.N, l.q, g);
-    // part [B * chunks][C * N of dA, C of dD, C of the bias]
-    float* part = a.part + ((long long)l.b * a.chunks + chunk) * a.C * (a.N + 2);
-    store_states<P>(part + (long long)l.c * a.N, a.N, l.q, dA);
-    if (l.q == 0) {
-      part[(long long)a.C * a.N + l.c] = dD;
-      part[(long long)a.C * (a.N + 1) + l.c] = dbias;
+  } else {
+    __syncthreads();
+    put_part(t_begin, buf ^ 1);
+    dD = quad_sum(dD);
+    dbias = quad_sum(dbias);
+    if (l.live) {
+      if (a.d_state_in && chunk == 0) store_states<P>(a.d_state_in + bC * a.N, a.N, l.q, g);
+      // part [B * chunks][C * N of dA, C of dD, C of the bias]
+      float* part = a.part + ((long long)l.b * a.chunks + chunk) * a.C * (a.N + 2);
+      store_states<P>(part + (long long)l.c * a.N, a.N, l.q, dA);
+      if (l.q == 0) {
+        part[(long long)a.C * a.N + l.c] = dD;
+        part[(long long)a.C * (a.N + 1) + l.c] = dbias;
+      }
     }
   }
 }
@@ -550,6 +620,9 @@ struct ScanGradients {
   }
 };
 
+#ifndef SCAN_WAVES
+#define SCAN_WAVES 8192
+#endif
 struct ScanShape {
   int P, groups, chunk, chunks;
 };
@@ -561,7 +634,7 @@ ScanShape scan_shape(int B, int T, int C, int N) {
   s.P = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
   s.groups = (C + 63) / 64;
   const long long waves = (long long)B * s.groups * 4;
-  long long chunks = (2048 + waves - 1) / waves;
+  long long chunks = waves >= 2048 ? 1 : (SCAN_WAVES + waves - 1) / waves;
   if (chunks > T / 64) chunks = T / 64;
   if (chunks < 1) chunks = 1;
   const int per = (int)((T + chunks - 1) / chunks);
@@ -611,7 +684,7 @@ extern "C" {
 
 size_t slamhip_selective_scan_kept_floats(int B, int T, int C, int N) {
   if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
-  const int tb = block_steps(scan_shape(B, T, C, N).P);
+  const int tb = kept_steps(scan_shape(B, T, C, N).P);
   return (size_t)B * ((T + tb - 1) / tb) * C * N;
 }
 

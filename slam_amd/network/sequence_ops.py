@@ -181,7 +181,7 @@ def causal_conv_bwd(dy, x, weight, bias, dx, dweight, dbias=None, state_in=None,
 
 
 def selective_scan_kept_states(B, T, C, N, device):
-    """The buffer in which selective_scan_fwd keeps states for selective_scan_bwd (every 16 steps, 8 for N > 16)."""
+    """The buffer in which selective_scan_fwd keeps states for selective_scan_bwd (every 16 steps, 8 for N > 8)."""
     return torch.empty(capi.load().slamhip_selective_scan_kept_floats(B, T, C, N), dtype=F32, device=device)
 
 

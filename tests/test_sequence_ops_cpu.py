@@ -99,7 +99,7 @@ def test_selective_scan_refusals():
     refused(E_ARG, "dz", b, *other(3, None))
     refused(E_ARG, "null", b, *other(10, None))
     refused(E_ARG, "workspace", b, *other(29, 0))
-    assert lib.slamhip_selective_scan_kept_floats(2, 33, 5, 16) == 2 * 3 * 5 * 16
+    assert lib.slamhip_selective_scan_kept_floats(2, 33, 5, 8) == 2 * 3 * 5 * 8
     assert lib.slamhip_selective_scan_kept_floats(2, 33, 5, 32) == 2 * 5 * 5 * 32
 
 

@@ -48,7 +48,7 @@ def test_quantize_and_product_refusals():
     g = "slamhip_gemm_nt_fp8"
     refused(E_ARG, "K >= 1", g, P, P, P, P, 1, 1, 0, P, None)
     refused(E_SIZE, "multiple of 16", g, P, P, P, P, 1, 1, 24, P, None)
-    refused(E_SIZE, "4 GB", g, P, P, P, P, 1 << 20, 1, 4096, P, None)
+    refused(E_SIZE, "2 GB", g, P, P, P, P, 1 << 20, 1, 4096, P, None)
     refused(E_ARG, "null", g, P, None, P, P, 1, 1, 16, P, None)
     refused(E_ARG, "aligned", g, ctypes.c_void_p(4104), P, P, P, 1, 1, 16, P, None)
     assert capi.load().slamhip_gemm_nt_fp8(None, None, None, None, 0, 8, 16, None, None) == 0

@@ -22,12 +22,6 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-#ifndef GEMM_BIG
-#define GEMM_BIG 192
-#endif
-#ifndef GEMM_SMALL
-#define GEMM_SMALL 64, 64, 2, 2
-#endif
 struct GemmArgs {
   const uint8_t *a, *b;
   const float *sa, *sb;
@@ -63,21 +57,29 @@ constexpr unsigned kBeyond = 0x80000000u;   // an offset past every operand, whi
 
 typedef const float __attribute__((address_space(4))) ConstFloat;
 
+// until at most N of the wave's loads are under way, and none of its reads of shared memory
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
 // floats that a wave reads alike and no kernel writes meanwhile: scalar loads
 __device__ __forceinline__ ConstFloat* uniform_floats(const float* p) { return (ConstFloat*)p; }
 
-// BM x BN outputs a workgroup, WM x WN waves; both operands' 128-deep slices and the rows' scales go from memory straight into
-// shared memory (two buffers).  A slice's row is eight 16-byte chunks, chunk c of row r at place c ^ (r & 7): the rows that a
+// BM x BN outputs a workgroup, KW groups of WM x WN waves that take every KW-th block of k and meet in shared memory at the end;
+// both operands' 128-deep slices and the rows' scales go from memory straight into shared memory (NS buffers of KW slices).  A slice's row is eight 16-byte chunks, chunk c of row r at place c ^ (r & 7): the rows that a
 // fragment read touches at once lie in different banks.  Chunks beyond the matrix are given an address beyond the buffer: they
 // arrive as zeros.  Per block of k a wave does TM x TN matrix instructions; the multiply-adds of one row of tiles are issued
 // behind the matrix instructions of the next, so that neither waits for the other.
-template <int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) gemm_fp8_kernel(GemmArgs p) {
-  constexpr int kWaves = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, kLoadA = BM / 8 / kWaves, kLoadB = BN / 8 / kWaves;
+template <int BM, int BN, int WM, int WN, int NS, int KW>
+__global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs p) {
+  constexpr int kWaves = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, kLoadA = BM / 8 / kWaves, kLoadB = BN / 8 / kWaves, kLoads = kLoadA + kLoadB;
   constexpr int kSlice = (BM + BN) * 128, kScales = BM * 16;
-  static_assert(128 % (BN / WN) == 0 && BM % 64 == 0 && BM / 64 <= kWaves, "a wave's columns share a scale");
-  __shared__ __align__(1024) uint8_t sh[2 * (kSlice + kScales)];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  static_assert(NS >= 2 && NS <= 4 && (KW == 1 || KW == 2) && 128 % (BN / WN) == 0 && BM % 64 == 0 && BM / 64 <= kWaves, "a wave's columns share a scale");
+  __shared__ __align__(1024) uint8_t sh[NS * KW * kSlice + 4 * kScales];
+  static_assert(KW == 1 || NS * KW * kSlice >= BM * BN * 4, "the groups' sums meet where the slices were");
+  const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = all_waves % kWaves, kg = all_waves / kWaves;
   // Workgroups of one XCD (every eighth) take neighbouring tiles, eight rows of tiles at a time: they share operands in its L2.
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, total = tiles_m * tiles_n;
   const int per_xcd = (total + 7) / 8, work = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
@@ -95,10 +97,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_fp8_kernel(GemmArgs p) {
   const unsigned off_a = (unsigned)(m0 + wave * 8 + lrow) * (unsigned)p.K + lchunk * 16;
   const unsigned off_b = (unsigned)(n0 + wave * 8 + lrow) * (unsigned)p.K + lchunk * 16;
   const unsigned off_s = (unsigned)(m0 + wave * 64 + lane) * (unsigned)p.KB * 4;
-  auto load = [&](int kb, int buf) {
+  auto load = [&](int it, int buf) {
+    const int kb = it * KW + kg;
     const bool in = kb * 128 + lchunk * 16 < p.K;
     const unsigned va = in ? off_a : kBeyond, vb = in ? off_b : kBeyond;
-    uint8_t* to = sh + buf * kSlice;
+    uint8_t* to = sh + (buf * KW + kg) * kSlice;
 #pragma unroll
     for (int i = 0; i < kLoadA; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(to + (i * kWaves + wave) * 1024), 16, va, kb * 128 + i * kWaves * 8 * p.K, 0, 0);
@@ -108,9 +111,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_fp8_kernel(GemmArgs p) {
   };
   // The rows' scales come for four blocks of k at a time, 16 bytes a row: a row's scales are one after the other, and a load of one
   // for each row touches as many lines of memory (331 instead of 299 us at 8192 x 8192 x 4096).
-  uint8_t* const scales = sh + 2 * kSlice;
+  uint8_t* const scales = sh + NS * KW * kSlice;
   auto load_scales = [&](int four) {
-    if (wave < BM / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(scales + (four & 1) * kScales + wave * 1024), 16, off_s, four * 16, 0, 0);
+    if (all_waves < BM / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(scales + (four & 3) * kScales + wave * 1024), 16, off_s, four * 16, 0, 0);
   };
   const int frow = lane & 15, g = lane >> 4;
   const int c0 = frow * 128 + (g ^ (frow & 7)) * 16, c1 = frow * 128 + ((g + 4) ^ (frow & 7)) * 16;
@@ -123,25 +126,33 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_fp8_kernel(GemmArgs p) {
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{};
-  load(0, 0);
   load_scales(0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  load_scales(1);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) load(i, i);
+  wait_loads<(NS - 1) * kLoads>();
   __syncthreads();
-  load(1, 1);
   i32x8 fb[TN], fa[2];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) fb[j] = fragment(sh + (BM + wn + j * 16) * 128);
-  fa[0] = fragment(sh + wm * 128);
+  for (int j = 0; j < TN; ++j) fb[j] = fragment(sh + kg * kSlice + (BM + wn + j * 16) * 128);
+  fa[0] = fragment(sh + kg * kSlice + wm * 128);
   // The buffers change hands one row of tiles before a block's end: by then its fragments are all in registers, and while the next
   // block's first fragments are read (a column's as soon as its registers are free) the matrix unit has that row to work on.
   // The loop has no branch: behind the last block zeros are brought and not used.
-  for (int kb = 0; kb < p.KB; ++kb) {
-    const uint8_t* base = sh + (kb & 1) * kSlice;
-    const uint8_t* other = sh + ((kb & 1) ^ 1) * kSlice;
-    const float sb = sbp[kb];
+  int buf = 0;
+  float sb_next = sbp[min(kg, p.KB - 1)];
+  for (int it = 0; it * KW < p.KB; ++it) {
+    const int kb = it * KW + kg, next_buf = buf + 1 == NS ? 0 : buf + 1;
+    const uint8_t* base = sh + (buf * KW + kg) * kSlice;
+    const uint8_t* other = sh + (next_buf * KW + kg) * kSlice;
+    const float sb = sb_next;
+    sb_next = sbp[min(kb + KW, p.KB - 1)];
     float s[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) s[i] = *reinterpret_cast<const float*>(scales + (kb >> 2 & 1) * kScales + (wm + i * 16 + frow) * 16 + (kb & 3) * 4) * sb;
+    for (int i = 0; i < TM; ++i) s[i] = *reinterpret_cast<const float*>(scales + (kb >> 2 & 3) * kScales + (wm + i * 16 + frow) * 16 + (kb & 3) * 4) * sb;
+    if (KW > 1 && kb >= p.KB)   // the last round of a group that has no block left
+#pragma unroll
+      for (int i = 0; i < TM; ++i) s[i] = 0.0f;
     f32x4 d[2][2];
     // tiles in pairs: the multiply-adds of a pair are issued behind the matrix instructions of the next
     auto add = [&](int pair) {
@@ -153,9 +164,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_fp8_kernel(GemmArgs p) {
     for (int i = 0; i < TM; ++i) {
       if (i + 1 < TM) fa[(i + 1) & 1] = fragment(base + (wm + (i + 1) * 16) * 128);
       if (i == TM - 1) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();   // slice kb + 1 has arrived for all waves, slice kb has been read by all
-        load(kb + 2, kb & 1);
+        wait_loads<(NS - 2) * kLoads>();
+        __syncthreads();   // the next slice has arrived for all waves, this one has been read by all
+        load(it + NS, buf);
       }
 #pragma unroll
       for (int j = 0; j < TN; j += 2) {
@@ -176,9 +187,22 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_fp8_kernel(GemmArgs p) {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[i][j]));
-    if ((kb & 3) == 1) load_scales((kb >> 2) + 1);   // two blocks before they are read
+    // two fours ahead: before the last wait in front of their first use two slices are asked for, as many as may be under way then
+    if ((it * KW & 3) == 0) load_scales((it * KW >> 2) + 2);
+    buf = next_buf;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is under way to shared memory when the workgroup ends
+  if constexpr (KW > 1) {
+    f32x4* const sums = reinterpret_cast<f32x4*>(sh) + (wave * TM * TN) * 64 + lane;
+    __syncthreads();
+    if (kg == 1)
+#pragma unroll
+      for (int i = 0; i < TM * TN; ++i) sums[i * 64] = acc[i / TN][i % TN];
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int i = 0; i < TM * TN; ++i) acc[i / TN][i % TN] += sums[i * 64];
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -223,11 +247,11 @@ __global__ void __launch_bounds__(256) gemm_fp8_rows_kernel(GemmArgs p) {
   }
 }
 
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int NS, int KW>
 int gemm_tiles(const GemmArgs& p, hipStream_t s) {
   const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   SLAMHIP_REQUIRE(tiles < (1 << 22), SLAMHIP_E_SIZE, "gemm_nt_fp8: too many tiles");
-  hipLaunchKernelGGL((gemm_fp8_kernel<BM, BN, WM, WN>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), 0, s, p);
+  hipLaunchKernelGGL((gemm_fp8_kernel<BM, BN, WM, WN, NS, KW>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN * KW), 0, s, p);
   SLAMHIP_HIP(hipGetLastError());
   return SLAMHIP_OK;
 }
@@ -244,9 +268,16 @@ int gemm(const GemmArgs& p, hipStream_t s) {
     SLAMHIP_HIP(hipGetLastError());
     return SLAMHIP_OK;
   }
-  const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (tiles >= GEMM_BIG) return gemm_tiles<256, 256, 2, 4>(p, s);
-  return gemm_tiles<GEMM_SMALL>(p, s);
+  // The largest tiles that still give most of the 256 CUs one.  Smaller ones read operands more often, larger ones leave CUs idle;
+  // two groups of waves (KW = 2) where a CU has one workgroup.  us, 256^2 / 128^2 / 128^2 KW / 64 x 128 KW / 64^2 KW:
+  // 4096x4096x4096 68/83/93/115/153, 2048x4096x4096 59/42/48/59/77, 1024x4096x4096 57/28/26/31/40, 777x2056x4096 54/25/22/16/21,
+  // 1024x1024x4096 56/25/22/16/12.
+  auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  if (tiles(256, 256) >= 192) return gemm_tiles<256, 256, 2, 4, 2, 1>(p, s);
+  if (tiles(128, 128) > 256) return gemm_tiles<128, 128, 2, 2, 2, 1>(p, s);
+  if (tiles(128, 128) > 128) return gemm_tiles<128, 128, 2, 2, 2, 2>(p, s);
+  if (tiles(64, 128) > 128) return gemm_tiles<64, 128, 2, 2, 3, 2>(p, s);
+  return gemm_tiles<64, 64, 2, 2, 4, 2>(p, s);
 }
 
 }  // namespace

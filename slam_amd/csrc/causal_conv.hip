@@ -3,7 +3,7 @@
 //   pre[b,t,c] = bias[c] + sum_k w[c,k] xp[b,t+k,c],  y = pre sigmoid(pre)      xp = K - 1 rows of state, then x
 //   backward: d = dy silu'(pre),  dxp[p] = sum_k w[k] d[p-k],  dw[c,k] = sum d[t] xp[t+k],  dbias = sum d
 //
-// A thread walks one octet of channels down a run of time steps with the last K rows in registers, so a row is read from memory
+// A thread walks a few channels down a run of time steps with the last K rows in registers, so a row is read from memory
 // once but for the K - 1 rows in front of a run (and, backward, as many behind it).  Nothing but the bytes bounds this.
 #include <hip/hip_runtime.h>
 
@@ -21,17 +21,18 @@ struct ConvArgs {
   const int* lengths;
   long long xb, xt, yb, yt, dyb, dyt, dxb, dxt;   // strides of a sequence and of a time step, in elements
   int T, C, run, runs, silu;
-  int lx_log2;   // a workgroup is 2^lx_log2 octets by 256 / 2^lx_log2 runs
+  int lx_log2;   // a workgroup is 2^lx_log2 threads along the channels by 256 / 2^lx_log2 runs
 };
 
 struct Place {
   int c, n, run, t0;
 };
 
+template <int V>
 __device__ __forceinline__ Place conv_place(const ConvArgs& a) {
   const int lx = 1 << a.lx_log2;
   Place p;
-  p.c = (blockIdx.x * lx + (threadIdx.x & (lx - 1))) * 8;
+  p.c = (blockIdx.x * lx + (threadIdx.x & (lx - 1))) * V;
   p.n = a.C - p.c;
   p.run = blockIdx.y * (256 >> a.lx_log2) + (threadIdx.x >> a.lx_log2);
   p.t0 = p.run * a.run;
@@ -45,64 +46,68 @@ __device__ __forceinline__ int conv_length(const ConvArgs& a, int b) {
 }
 
 // row `t` of a sequence: state rows in front of it, zeros where it has neither
-template <typename T, int K>
-__device__ __forceinline__ f32x8 conv_row(const ConvArgs& a, const T* x, const T* state, int t, int len, int c, int n) {
-  if (t >= 0) return t < len ? load8(x + t * a.xt + c, n) : f32x8{};
-  return state ? load8(state + (long long)(t + K - 1) * a.C + c, n) : f32x8{};
+template <typename T, int K, int V>
+__device__ __forceinline__ floats<V> conv_row(const ConvArgs& a, const T* x, const T* state, int t, int len, int c, int n) {
+  if (t >= 0) return t < len ? loadv<V>(x + t * a.xt + c, n) : floats<V>{};
+  return state ? loadv<V>(state + (long long)(t + K - 1) * a.C + c, n) : floats<V>{};
 }
 
-template <int K>
-__device__ __forceinline__ void conv_weights(const ConvArgs& a, int c, int n, f32x8 (&w)[K], f32x8& bias) {
+// a thread's filters lie one behind the other: V K floats
+template <int K, int V>
+__device__ __forceinline__ void conv_weights(const ConvArgs& a, int c, int n, floats<V> (&w)[K], floats<V>& bias) {
+  floats<V> flat[K];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    bias[j] = a.bias && j < n ? a.bias[c + j] : 0.0f;
+  for (int k = 0; k < K; ++k) flat[k] = loadv<V>(a.w + (long long)c * K + k * V, n * K - k * V);
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][j] = j < n ? a.w[(long long)(c + j) * K + k] : 0.0f;
-  }
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][j] = flat[(j * K + k) / V][(j * K + k) % V];
+  bias = floats<V>{};
+  if (a.bias) bias = loadv<V>(a.bias + c, n);
 }
 
-template <typename T, int K>
+template <typename T, int K, int V>
 __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
-  const Place p = conv_place(a);
+  const Place p = conv_place<V>(a);
   const int b = blockIdx.z, len = conv_length(a, b);
   if (p.n <= 0 || p.run >= a.runs) return;
   const T* x = (const T*)a.x + b * a.xb;
   T* y = (T*)a.y + b * a.yb;
   const T* state = a.state_in ? (const T*)a.state_in + (long long)b * (K - 1) * a.C : nullptr;
-  f32x8 w[K], bias, win[K];
-  conv_weights<K>(a, p.c, p.n, w, bias);
+  floats<V> w[K], bias, win[K];
+  conv_weights<K, V>(a, p.c, p.n, w, bias);
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) win[k] = conv_row<T, K>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
+  for (int k = 0; k < K - 1; ++k) win[k] = conv_row<T, K, V>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
   if (p.run == 0 && a.state_out) {   // win holds the state: it may be written over from here on
     T* out = (T*)a.state_out + (long long)b * (K - 1) * a.C;
 #pragma unroll
     for (int i = 0; i < K - 1; ++i) {
-      f32x8 v{};
-      if (len + i >= K - 1) v = load8(x + (len + i - (K - 1)) * a.xt + p.c, p.n);
+      floats<V> v{};
+      if (len + i >= K - 1) v = loadv<V>(x + (len + i - (K - 1)) * a.xt + p.c, p.n);
 #pragma unroll
       for (int k = 0; k < K - 1; ++k)
         if (len + i == k) v = win[k];
-      store8(out + (long long)i * a.C + p.c, v, p.n);
+      storev<V>(out + (long long)i * a.C + p.c, v, p.n);
     }
   }
   const int t1 = min(p.t0 + a.run, a.T);
   for (int t = p.t0; t < t1; t += 4) {
-    f32x8 next[4];
+    floats<V> next[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) next[i] = t + i < t1 ? conv_row<T, K>(a, x, nullptr, t + i, len, p.c, p.n) : f32x8{};
+    for (int i = 0; i < 4; ++i) next[i] = t + i < t1 ? conv_row<T, K, V>(a, x, nullptr, t + i, len, p.c, p.n) : floats<V>{};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       win[K - 1] = next[i];
-      f32x8 v = bias;
+      floats<V> v = bias;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf(w[k][j], win[k][j], v[j]);
+        for (int j = 0; j < V; ++j) v[j] = fmaf(w[k][j], win[k][j], v[j]);
       if (a.silu)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= sigmoid_(v[j]);
-      if (t + i >= len) v = f32x8{};
-      if (t + i < t1) store8(y + (t + i) * a.yt + p.c, v, p.n);
+        for (int j = 0; j < V; ++j) v[j] *= sigmoid_(v[j]);
+      if (t + i >= len) v = floats<V>{};
+      if (t + i < t1) storev<V>(y + (t + i) * a.yt + p.c, v, p.n);
 #pragma unroll
       for (int k = 0; k < K - 1; ++k) win[k] = win[k + 1];
     }
@@ -110,15 +115,15 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
 }
 
 // part [sequence][group of runs][K + 1][C]: dw and dbias of a workgroup's runs
-template <typename T, int K>
+template <typename T, int K, int V>
 __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
-  __shared__ float sh[256 * 8];
-  const Place p = conv_place(a);
+  __shared__ float sh[256 * V];
+  const Place p = conv_place<V>(a);
   const int b = blockIdx.z, len = conv_length(a, b);
   const bool live = p.n > 0 && p.run < a.runs;
-  f32x8 dw[K], db{};
+  floats<V> dw[K], db{};
 #pragma unroll
-  for (int k = 0; k < K; ++k) dw[k] = f32x8{};
+  for (int k = 0; k < K; ++k) dw[k] = floats<V>{};
   if (live) {
     const T* x = (const T*)a.x + b * a.xb;
     const T* dy = (const T*)a.dy + b * a.dyb;
@@ -127,39 +132,39 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
     const T* state = a.state_in ? (const T*)a.state_in + sbase : nullptr;
     const T* d_out = a.d_state_out ? (const T*)a.d_state_out + sbase : nullptr;
     T* d_in = a.d_state_in ? (T*)a.d_state_in + sbase : nullptr;
-    f32x8 w[K], bias, win[K], d[K];
-    conv_weights<K>(a, p.c, p.n, w, bias);
+    floats<V> w[K], bias, win[K], d[K];
+    conv_weights<K, V>(a, p.c, p.n, w, bias);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      d[k] = f32x8{};   // d[k] is the gradient at pre of step t - (K - 1) + k
-      if (k < K - 1) win[k] = conv_row<T, K>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
+      d[k] = floats<V>{};   // d[k] is the gradient at pre of step t - (K - 1) + k
+      if (k < K - 1) win[k] = conv_row<T, K, V>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
     }
     const int t1 = min(p.t0 + a.run, a.T);
     const int first = p.run == 0 ? -(K - 1) : p.t0;   // the first run's rows begin with the state's
     for (int t = p.t0; t < t1 + K - 1; t += 2) {
-      f32x8 nx[2], ny[2];
+      floats<V> nx[2], ny[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bool in = t + i < t1 + K - 1 && t + i < len;
-        nx[i] = in ? load8(x + (t + i) * a.xt + p.c, p.n) : f32x8{};
-        ny[i] = in ? load8(dy + (t + i) * a.dyt + p.c, p.n) : f32x8{};
+        nx[i] = in ? loadv<V>(x + (t + i) * a.xt + p.c, p.n) : floats<V>{};
+        ny[i] = in ? loadv<V>(dy + (t + i) * a.dyt + p.c, p.n) : floats<V>{};
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int now = t + i;
         if (now < t1 + K - 1) {
           win[K - 1] = nx[i];
-          f32x8 g{};
+          floats<V> g{};
           if (now < len) {
             g = ny[i];
             if (a.silu) {
-              f32x8 pre = bias;
+              floats<V> pre = bias;
 #pragma unroll
               for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) pre[j] = fmaf(w[k][j], win[k][j], pre[j]);
+                for (int j = 0; j < V; ++j) pre[j] = fmaf(w[k][j], win[k][j], pre[j]);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
+              for (int j = 0; j < V; ++j) {
                 const float s = sigmoid_(pre[j]);
                 g[j] *= s * fmaf(pre[j], 1.0f - s, 1.0f);
               }
@@ -171,22 +176,22 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) dw[k][j] = fmaf(g[j], win[k][j], dw[k][j]);
+              for (int j = 0; j < V; ++j) dw[k][j] = fmaf(g[j], win[k][j], dw[k][j]);
           }
           const int row = now - (K - 1);
           if (row >= first) {
-            f32x8 v{};
+            floats<V> v{};
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = fmaf(w[k][j], d[K - 1 - k][j], v[j]);
+              for (int j = 0; j < V; ++j) v[j] = fmaf(w[k][j], d[K - 1 - k][j], v[j]);
             const int i_state = row - len + K - 1;   // row of the state that leaves
-            if (d_out && i_state >= 0 && i_state < K - 1) v += load8(d_out + (long long)i_state * a.C + p.c, p.n);
+            if (d_out && i_state >= 0 && i_state < K - 1) v += loadv<V>(d_out + (long long)i_state * a.C + p.c, p.n);
             if (row >= 0) {
-              if (row >= len) v = f32x8{};
-              store8(dx + row * a.dxt + p.c, v, p.n);
+              if (row >= len) v = floats<V>{};
+              storev<V>(dx + row * a.dxt + p.c, v, p.n);
             } else if (d_in) {
-              store8(d_in + (long long)(row + K - 1) * a.C + p.c, v, p.n);
+              storev<V>(d_in + (long long)(row + K - 1) * a.C + p.c, v, p.n);
             }
           }
 #pragma unroll
@@ -203,15 +208,15 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
   float* part = a.part + ((long long)b * gridDim.y + blockIdx.y) * (K + 1) * a.C;
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
-    const f32x8 v = k < K ? dw[k < K ? k : 0] : db;
+    const floats<V> v = k < K ? dw[k < K ? k : 0] : db;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sh[j * 256 + threadIdx.x] = v[j];
+    for (int j = 0; j < V; ++j) sh[j * 256 + threadIdx.x] = v[j];
     __syncthreads();
-    for (int i = threadIdx.x; i < lx * 8; i += 256) {   // i = channel within the workgroup's
+    for (int i = threadIdx.x; i < lx * V; i += 256) {   // i = channel within the workgroup's
       float s = 0.0f;
-      for (int r = 0; r < ly; ++r) s += sh[(i & 7) * 256 + r * lx + (i >> 3)];
-      const int c = blockIdx.x * lx * 8 + i;
+      for (int r = 0; r < ly; ++r) s += sh[i % V * 256 + r * lx + i / V];
+      const int c = blockIdx.x * lx * V + i;
       if (c < a.C) part[(long long)k * a.C + c] = s;
     }
   }
@@ -221,40 +226,55 @@ struct ConvShape {
   int run, runs, lx_log2, gx, gy;
 };
 
-// Runs are as long as leaves about eight waves a SIMD (fewer rows are read twice); short sequences take shorter ones.
-ConvShape conv_shape(int B, int T, int C, int longest, int align) {
+#ifndef CONV_VF
+#define CONV_VF 8
+#endif
+#ifndef CONV_VB
+#define CONV_VB 4
+#endif
+#ifndef CONV_WF
+#define CONV_WF 8192
+#endif
+#ifndef CONV_WB
+#define CONV_WB 8192
+#endif
+constexpr int kFwdChannels = CONV_VF, kBwdChannels = CONV_VB;
+
+// Runs are as long as leaves `waves` waves (fewer rows are read twice); short sequences take shorter ones.
+ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int waves) {
   ConvShape s;
-  const int octets = (C + 7) / 8;
-  s.lx_log2 = 0;
-  while (s.lx_log2 < 6 && (1 << s.lx_log2) < octets) ++s.lx_log2;
-  s.gx = (octets + (1 << s.lx_log2) - 1) >> s.lx_log2;
-  const long long rows_per_thread = (long long)B * T * octets / (8192LL * 64);
+  const int across = (C + V - 1) / V;
+  const long long rows_per_thread = (long long)B * T * across / (waves * 64LL);
   long long run = (rows_per_thread + align - 1) / align * align;
   if (run < align) run = align;
   if (run > longest) run = longest;
   s.run = (int)run;
   s.runs = T > 0 ? (T + s.run - 1) / s.run : 1;
+  s.lx_log2 = 0;
+  while (s.lx_log2 < 8 && (1 << s.lx_log2) < across && (s.lx_log2 < 6 || (256 >> s.lx_log2) > s.runs)) ++s.lx_log2;
+  s.gx = (across + (1 << s.lx_log2) - 1) >> s.lx_log2;
   const int ly = 256 >> s.lx_log2;
   s.gy = (s.runs + ly - 1) / ly;
   return s;
 }
 
-constexpr int kFwdLongest = 16, kFwdAlign = 4, kBwdLongest = 64, kBwdAlign = 8;
+ConvShape fwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kFwdChannels, 16, 4, CONV_WF); }
+ConvShape bwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kBwdChannels, 64, 8, CONV_WB); }
 
 template <typename T>
 int conv_fwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {
-  if (K == 2) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 2>), grid, dim3(256), 0, s, a);
-  if (K == 3) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 3>), grid, dim3(256), 0, s, a);
-  if (K == 4) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 4>), grid, dim3(256), 0, s, a);
+  if (K == 2) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 2, kFwdChannels>), grid, dim3(256), 0, s, a);
+  if (K == 3) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 3, kFwdChannels>), grid, dim3(256), 0, s, a);
+  if (K == 4) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 4, kFwdChannels>), grid, dim3(256), 0, s, a);
   SLAMHIP_HIP(hipGetLastError());
   return SLAMHIP_OK;
 }
 
 template <typename T>
 int conv_bwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {
-  if (K == 2) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 2>), grid, dim3(256), 0, s, a);
-  if (K == 3) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 3>), grid, dim3(256), 0, s, a);
-  if (K == 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 4>), grid, dim3(256), 0, s, a);
+  if (K == 2) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 2, kBwdChannels>), grid, dim3(256), 0, s, a);
+  if (K == 3) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 3, kBwdChannels>), grid, dim3(256), 0, s, a);
+  if (K == 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 4, kBwdChannels>), grid, dim3(256), 0, s, a);
   SLAMHIP_HIP(hipGetLastError());
   return SLAMHIP_OK;
 }
@@ -290,7 +310,7 @@ int slamhip_causal_conv_fwd(const void* x, const long long* strides, const float
   ConvArgs a{};
   a.x = x, a.w = weight, a.bias = bias, a.state_in = state_in, a.y = y, a.state_out = state_out, a.lengths = lengths;
   if (strides) a.xb = strides[0], a.xt = strides[1], a.yb = strides[2], a.yt = strides[3];
-  const ConvShape g = conv_shape(B, T, C, kFwdLongest, kFwdAlign);
+  const ConvShape g = fwd_shape(B, T, C);
   a.T = T, a.C = C, a.run = g.run, a.runs = g.runs, a.silu = silu, a.lx_log2 = g.lx_log2;
   const dim3 grid(g.gx, g.gy, B);
   SLAMHIP_REQUIRE(g.gy <= 65535, SLAMHIP_E_SIZE, "causal_conv_fwd: too many steps");
@@ -299,7 +319,7 @@ int slamhip_causal_conv_fwd(const void* x, const long long* strides, const float
 
 size_t slamhip_causal_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
   if (B <= 0 || C <= 0 || T < 0 || K < 2) return 0;
-  return (size_t)B * conv_shape(B, T, C, kBwdLongest, kBwdAlign).gy * (K + 1) * C * sizeof(float);
+  return (size_t)B * bwd_shape(B, T, C).gy * (K + 1) * C * sizeof(float);
 }
 
 int slamhip_causal_conv_bwd(const void* dy, const void* x, const long long* strides, const float* weight, const float* bias,
@@ -313,7 +333,7 @@ int slamhip_causal_conv_bwd(const void* dy, const void* x, const long long* stri
                   "causal_conv_bwd: null pointer");
   SLAMHIP_REQUIRE(workspace_bytes >= slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K), SLAMHIP_E_ARG, "causal_conv_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
-  const ConvShape g = conv_shape(B, T, C, kBwdLongest, kBwdAlign);
+  const ConvShape g = bwd_shape(B, T, C);
   if (B > 0) {
     ConvArgs a{};
     a.x = x, a.dy = dy, a.w = weight, a.bias = bias, a.state_in = state_in, a.d_state_out = d_state_out, a.lengths = lengths;

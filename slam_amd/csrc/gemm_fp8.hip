@@ -209,33 +209,51 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
     for (int j = 0; j < TN; ++j) store_out(p, m0 + wm + i * 16 + frow, n0 + wn + j * 16 + g * 4, acc[i][j]);
 }
 
-// Few rows: the weights are read once, straight into registers; a workgroup's waves take every kWaves-th block of k for the same
-// 16 columns and meet in shared memory.
-template <int TM>
-__global__ void __launch_bounds__(256) gemm_fp8_rows_kernel(GemmArgs p) {
-  constexpr int kWaves = 4;
+// Few rows: the weights are read once, straight into registers; a workgroup's waves take every eighth block of k for the same 16
+// columns and meet in shared memory.  U blocks are loaded at once: the whole of K = 4096 for up to 16 rows.
+template <int TM, int U>
+__global__ void __launch_bounds__(512) gemm_fp8_rows_kernel(GemmArgs p) {
+  constexpr int kWaves = 8;
   __shared__ f32x4 sh[kWaves][TM][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n0 = blockIdx.x * 16, row = lane & 15, g = lane >> 4;
   const uint8_t* b = p.b + (long long)min(n0 + row, p.N - 1) * p.K;
+  ConstFloat* sbp = uniform_floats(p.sb + (long long)(n0 / 128) * p.KB);
+  const uint8_t* a[TM];
+  const float* sap[TM];
   f32x4 acc[TM];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) acc[i] = f32x4{};
-  for (int kb = wave; kb < p.KB; kb += kWaves) {
-    const int k0 = kb * 128 + g * 16, k1 = k0 + 64;
-    i32x4 z{};
-    const i32x8 fb = join(k0 < p.K ? *reinterpret_cast<const i32x4*>(b + k0) : z, k1 < p.K ? *reinterpret_cast<const i32x4*>(b + k1) : z);
-    const float sb = p.sb[(long long)(n0 / 128) * p.KB + kb];
+  for (int i = 0; i < TM; ++i) {
+    const int m = min(i * 16 + row, p.M - 1);   // rows beyond the last repeat it and are not stored
+    a[i] = p.a + (long long)m * p.K;
+    sap[i] = p.sa + (long long)m * p.KB;
+    acc[i] = f32x4{};
+  }
+  for (int kb0 = wave; kb0 < p.KB; kb0 += kWaves * U) {
+    i32x8 fb[U], fa[TM][U];
+    float sa[TM][U], sb[U];
+    const i32x4 zero{};
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int m = min(i * 16 + row, p.M - 1);   // rows beyond the last repeat it and are not stored
-      const uint8_t* a = p.a + (long long)m * p.K;
-      const i32x8 fa = join(k0 < p.K ? *reinterpret_cast<const i32x4*>(a + k0) : z, k1 < p.K ? *reinterpret_cast<const i32x4*>(a + k1) : z);
-      const float s = p.sa[(long long)m * p.KB + kb] * sb;
-      const f32x4 d = mfma_fp8(fb, fa);
+    for (int u = 0; u < U; ++u) {
+      const int kb = kb0 + u * kWaves, k0 = kb * 128 + g * 16, k1 = k0 + 64;
+      const bool in0 = k0 < p.K, in1 = k1 < p.K;
+      fb[u] = join(in0 ? *reinterpret_cast<const i32x4*>(b + k0) : zero, in1 ? *reinterpret_cast<const i32x4*>(b + k1) : zero);
+      sb[u] = kb < p.KB ? sbp[kb] : 0.0f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(d[r], s, acc[i][r]);
+      for (int i = 0; i < TM; ++i) {
+        fa[i][u] = join(in0 ? *reinterpret_cast<const i32x4*>(a[i] + k0) : zero, in1 ? *reinterpret_cast<const i32x4*>(a[i] + k1) : zero);
+        sa[i][u] = kb < p.KB ? sap[i][kb] : 0.0f;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const f32x4 d = mfma_fp8(fb[u], fa[i][u]);
+        const float s = sa[i][u] * sb[u];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(d[r], s, acc[i][r]);
+      }
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i) sh[wave][i][lane] = acc[i];
@@ -260,11 +278,11 @@ int gemm(const GemmArgs& p, hipStream_t s) {
   if (p.M <= 64) {
     const dim3 grid((p.N + 15) / 16);
     if (p.M <= 16)
-      hipLaunchKernelGGL((gemm_fp8_rows_kernel<1>), grid, dim3(256), 0, s, p);
+      hipLaunchKernelGGL((gemm_fp8_rows_kernel<1, 4>), grid, dim3(512), 0, s, p);
     else if (p.M <= 32)
-      hipLaunchKernelGGL((gemm_fp8_rows_kernel<2>), grid, dim3(256), 0, s, p);
+      hipLaunchKernelGGL((gemm_fp8_rows_kernel<2, 2>), grid, dim3(512), 0, s, p);
     else
-      hipLaunchKernelGGL((gemm_fp8_rows_kernel<4>), grid, dim3(256), 0, s, p);
+      hipLaunchKernelGGL((gemm_fp8_rows_kernel<4, 1>), grid, dim3(512), 0, s, p);
     SLAMHIP_HIP(hipGetLastError());
     return SLAMHIP_OK;
   }

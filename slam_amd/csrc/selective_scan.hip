@@ -321,6 +321,40 @@ __global__ void __launch_bounds__(256, 4) selective_scan_fwd_kernel(ScanArgs a) 
   }
 }
 
+// One step (T = 1): the state comes and goes, nothing is handed on.  No staging, no barrier, few registers: all waves of 32 x 4096
+// channels are on the chip at once.
+template <typename T, int P, bool Z>
+__global__ void __launch_bounds__(256) selective_scan_step_kernel(ScanArgs a) {
+  const Lane l = scan_lane(a);
+  if (!l.live) return;   // whole quads
+  const long long bC = (long long)l.b * a.C + l.c;
+  float h[P], A2[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) h[i] = 0.0f;
+  if (a.state_in) load_states<P>(a.state_in + bC * a.N, a.N, l.q, h);
+  float y = 0.0f;
+  if (l.len > 0) {
+    load_states<P>(a.A + (long long)l.c * a.N, a.N, l.q, A2);
+    const floats<P> Bv = loadv<P>((const T*)a.Bm + l.b * a.Bb + l.q * P, a.N - l.q * P);
+    const floats<P> Cv = loadv<P>((const T*)a.Cm + l.b * a.Cb + l.q * P, a.N - l.q * P);
+    const float u = (float)((const T*)a.u)[l.b * a.ub + l.c];
+    const float z = Z ? (float)((const T*)a.z)[l.b * a.zb + l.c] : 0.0f;
+    float dt = (float)((const T*)a.delta)[l.b * a.deltab + l.c] + (a.bias ? a.bias[l.c] : 0.0f);
+    if (a.softplus) dt = softplus_(dt, exp2_(-kLog2e * fabsf(dt)));
+    float inner = 0.0f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      h[i] = fmaf(exp2_(A2[i] * kLog2e * dt), h[i], dt * u * Bv[i]);
+      inner = fmaf(h[i], Cv[i], inner);
+    }
+    y = quad_sum(inner);
+    if (a.D) y = fmaf(a.D[l.c], u, y);
+    if (Z) y *= z * sigmoid_(z);
+  }
+  if (l.q == 0) ((T*)a.y)[l.b * a.yb + l.c] = (T)y;
+  if (a.state_out) store_states<P>(a.state_out + bC * a.N, a.N, l.q, h);
+}
+
 // v[p] (p < P) and w[p] summed over the wave's 16 channels (lanes of equal place in the quad).  Swapping halves (rows) of two
 // registers and adding them sums both at once, half a wave (a row) each; what is left are four channels of a row.
 template <int P>
@@ -673,6 +707,14 @@ ScanShape scan_shape(int B, int T, int C, int N) {
 template <typename T, int P>
 int scan_fwd(const ScanArgs& a, int groups, int B, hipStream_t s) {
   const dim3 grid(groups, a.chunks, B);
+  if (a.T == 1 && !a.kept) {
+    if (a.z)
+      hipLaunchKernelGGL((selective_scan_step_kernel<T, P, true>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((selective_scan_step_kernel<T, P, false>), grid, dim3(256), 0, s, a);
+    SLAMHIP_HIP(hipGetLastError());
+    return SLAMHIP_OK;
+  }
   // nothing follows the last chunk: its end is not asked for
   if (a.chunks > 1) hipLaunchKernelGGL((selective_scan_fwd_kernel<T, P, true, false>), dim3(groups, a.chunks - 1, B), dim3(256), 0, s, a);
   if (a.z)

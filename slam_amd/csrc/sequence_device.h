@@ -12,49 +12,54 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// Eight consecutive elements of a row, at the element's own alignment: gfx950 takes unaligned global accesses, so rows of odd
-// length and views at odd offsets use the same 16-byte loads as aligned ones.
-template <typename T>
-struct Packed8;
-template <>
-struct Packed8<float> {
-  typedef f32x8 __attribute__((aligned(4))) type;
+template <int V>
+struct Floats {
+  typedef float type __attribute__((ext_vector_type(V)));
 };
-template <>
-struct Packed8<__bf16> {
-  typedef bf16x8 __attribute__((aligned(2))) type;
+template <int V>
+using floats = typename Floats<V>::type;
+
+// V consecutive elements of a row, at the element's own alignment: gfx950 takes unaligned global accesses, so rows of odd length
+// and views at odd offsets use the same vector accesses as aligned ones.
+template <typename T, int V>
+struct Packed {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
 
-// valid >= 8: one vector access; fewer: element by element, the rest zero
-template <typename T>
-__device__ __forceinline__ f32x8 load8(const T* p, int valid) {
-  f32x8 v;
-  if (valid >= 8) {
-    const typename Packed8<T>::type raw = *reinterpret_cast<const typename Packed8<T>::type*>(p);
+// valid >= V: one vector access; fewer: element by element, the rest zero
+template <int V, typename T>
+__device__ __forceinline__ floats<V> loadv(const T* p, int valid) {
+  floats<V> v;
+  if (valid >= V) {
+    const typename Packed<T, V>::type raw = *reinterpret_cast<const typename Packed<T, V>::type*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
+    for (int i = 0; i < V; ++i) v[i] = (float)raw[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < valid ? (float)p[i] : 0.0f;
+    for (int i = 0; i < V; ++i) v[i] = i < valid ? (float)p[i] : 0.0f;
   }
   return v;
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, f32x8 v, int valid) {
-  if (valid >= 8) {
-    typename Packed8<T>::type raw;
+template <int V, typename T>
+__device__ __forceinline__ void storev(T* p, floats<V> v, int valid) {
+  if (valid >= V) {
+    typename Packed<T, V>::type raw;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = (T)v[i];
-    *reinterpret_cast<typename Packed8<T>::type*>(p) = raw;
+    for (int i = 0; i < V; ++i) raw[i] = (T)v[i];
+    *reinterpret_cast<typename Packed<T, V>::type*>(p) = raw;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < V; ++i)
       if (i < valid) p[i] = (T)v[i];
   }
 }
+
+template <typename T>
+__device__ __forceinline__ f32x8 load8(const T* p, int valid) { return loadv<8>(p, valid); }
+template <typename T>
+__device__ __forceinline__ void store8(T* p, f32x8 v, int valid) { storev<8>(p, v, valid); }
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float log2_(float v) { return __builtin_amdgcn_logf(v); }

@@ -20,12 +20,14 @@ _DTYPE = {F32: 0, BF16: 1}
 
 
 def _launch(device, name, *args):
-    lib = capi.load()
-    if device.index != torch.cuda.current_device():
+    # (torch.cuda.current_stream() makes an object of every call, 2 us; a launch takes 4)
+    fn = getattr(capi.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device != torch.cuda.current_device():
         with torch.cuda.device(device):
-            capi.check(getattr(lib, name)(*args, capi.current_stream()), name)
+            capi.check(fn(*args, stream), name)
     else:
-        capi.check(getattr(lib, name)(*args, capi.current_stream()), name)
+        capi.check(fn(*args, stream), name)
 
 
 def _bad(what, t, want):
@@ -34,9 +36,9 @@ def _bad(what, t, want):
 
 
 def _flat(t, dtype, shape, device, what):
-    """A contiguous tensor of this type and shape on `device`; its address."""
-    if t is None or t.dtype is not dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        _bad(what, t, "a contiguous %s tensor %s on %s" % (dtype, shape, device))
+    """A contiguous tensor of this type and shape on GPU `device`; its address."""
+    if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        _bad(what, t, "a contiguous %s tensor %s on cuda:%d" % (dtype, shape, device))
     return t.data_ptr()
 
 
@@ -45,16 +47,16 @@ def _opt(t, dtype, shape, device, what):
 
 
 def _matrix(t, what):
-    """(rows, columns, type code, device) of a contiguous float32 or bfloat16 GPU matrix."""
+    """(rows, columns, type code, device index) of a contiguous float32 or bfloat16 GPU matrix."""
     if t.dim() != 2 or t.dtype not in _DTYPE or not t.is_cuda or not t.is_contiguous() or t.shape[1] == 0:
         _bad(what, t, "a contiguous float32 or bfloat16 GPU matrix with columns")
-    return t.shape[0], t.shape[1], _DTYPE[t.dtype], t.device
+    return t.shape[0], t.shape[1], _DTYPE[t.dtype], t.get_device()
 
 
 def _seq(t, dtype, shape, device, what, out=False):
     """A sequence [B, T, C] of this type with unit stride over C; an output's rows may not overlap."""
-    if t is None or t.dtype is not dtype or tuple(t.shape) != shape or t.device != device:
-        _bad(what, t, "a %s tensor %s on %s" % (dtype, shape, device))
+    if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+        _bad(what, t, "a %s tensor %s on cuda:%d" % (dtype, shape, device))
     (B, T, C), (sb, st, sc) = shape, t.stride()
     if sc != 1 and C > 1:
         _bad(what, t, "unit stride over the last axis")
@@ -64,11 +66,11 @@ def _seq(t, dtype, shape, device, what, out=False):
 
 
 def _sequence(t, what):
-    """(B, T, C, type, device) of a float32 or bfloat16 GPU tensor [B, T, C]."""
+    """(B, T, C, type, device index) of a float32 or bfloat16 GPU tensor [B, T, C]."""
     if t.dim() != 3 or t.dtype not in _DTYPE or not t.is_cuda or t.shape[2] == 0:
         _bad(what, t, "a float32 or bfloat16 GPU tensor [B, T, C] with channels")
     B, T, C = t.shape
-    return B, T, C, t.dtype, t.device
+    return B, T, C, t.dtype, t.get_device()
 
 
 def _strides(*ts):
@@ -131,7 +133,7 @@ def gemm_nt_fp8(a8, a_scales, b8, b_scales, out):
     quantize_fp8 (or rms_norm_fwd) and quantize_fp8_blocks write.  K a multiple of 16."""
     if out.dim() != 2 or not out.is_cuda or a8.dim() != 2 or a8.shape[1] == 0:
         _bad("out", out, "a bfloat16 GPU matrix and operands with columns")
-    (M, N), K, dev = out.shape, a8.shape[1], out.device
+    (M, N), K, dev = out.shape, a8.shape[1], out.get_device()
     kb = (K + 127) // 128
     if K % 16 or a8.data_ptr() % 16 or b8.data_ptr() % 16:
         raise ValueError("gemm_nt_fp8: K must be a multiple of 16 and the operands 16-byte aligned, got K = %d" % K)

@@ -90,14 +90,21 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
       storev<V>(out + (long long)i * a.C + p.c, v, p.n);
     }
   }
-  const int t1 = min(p.t0 + a.run, a.T);
-  for (int t = p.t0; t < t1; t += 4) {
-    floats<V> next[4];
+  const int t1 = min(p.t0 + a.run, a.T), last = min(t1, len);
+  packed<T, V> next[4];
+  auto fetch = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) next[i] = t + i < t1 ? conv_row<T, K, V>(a, x, nullptr, t + i, len, p.c, p.n) : floats<V>{};
+    for (int i = 0; i < 4; ++i) next[i] = load_raw<V>(x + (t + i) * a.xt + p.c, t + i < last ? p.n : 0);
+  };
+  fetch(p.t0);
+  for (int t = p.t0; t < t1; t += 4) {
+    packed<T, V> now[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) now[i] = next[i];
+    if (t + 4 < t1) fetch(t + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      win[K - 1] = next[i];
+      win[K - 1] = to_floats<T, V>(now[i]);
       floats<V> v = bias;
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -117,6 +124,7 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
 // part [sequence][group of runs][K + 1][C]: dw and dbias of a workgroup's runs
 template <typename T, int K, int V>
 __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
+  constexpr int U = 2;   // rows under way
   __shared__ float sh[256 * V];
   const Place p = conv_place<V>(a);
   const int b = blockIdx.z, len = conv_length(a, b);
@@ -141,22 +149,29 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
     }
     const int t1 = min(p.t0 + a.run, a.T);
     const int first = p.run == 0 ? -(K - 1) : p.t0;   // the first run's rows begin with the state's
-    for (int t = p.t0; t < t1 + K - 1; t += 2) {
-      floats<V> nx[2], ny[2];
+    const int last = min(t1 + K - 1, len);
+    packed<T, V> next_x[U], next_y[U];
+    auto fetch = [&](int t) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool in = t + i < t1 + K - 1 && t + i < len;
-        nx[i] = in ? loadv<V>(x + (t + i) * a.xt + p.c, p.n) : floats<V>{};
-        ny[i] = in ? loadv<V>(dy + (t + i) * a.dyt + p.c, p.n) : floats<V>{};
+      for (int i = 0; i < U; ++i) {
+        next_x[i] = load_raw<V>(x + (t + i) * a.xt + p.c, t + i < last ? p.n : 0);
+        next_y[i] = load_raw<V>(dy + (t + i) * a.dyt + p.c, t + i < last ? p.n : 0);
       }
+    };
+    fetch(p.t0);
+    for (int t = p.t0; t < t1 + K - 1; t += U) {
+      packed<T, V> nx[U], ny[U];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < U; ++i) nx[i] = next_x[i], ny[i] = next_y[i];
+      if (t + U < t1 + K - 1) fetch(t + U);
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
         const int now = t + i;
         if (now < t1 + K - 1) {
-          win[K - 1] = nx[i];
+          win[K - 1] = to_floats<T, V>(nx[i]);
           floats<V> g{};
           if (now < len) {
-            g = ny[i];
+            g = to_floats<T, V>(ny[i]);
             if (a.silu) {
               floats<V> pre = bias;
 #pragma unroll
@@ -226,19 +241,7 @@ struct ConvShape {
   int run, runs, lx_log2, gx, gy;
 };
 
-#ifndef CONV_VF
-#define CONV_VF 8
-#endif
-#ifndef CONV_VB
-#define CONV_VB 4
-#endif
-#ifndef CONV_WF
-#define CONV_WF 8192
-#endif
-#ifndef CONV_WB
-#define CONV_WB 8192
-#endif
-constexpr int kFwdChannels = CONV_VF, kBwdChannels = CONV_VB;
+constexpr int kChannels = 4;   // a thread's; eight take 146 and 209 registers: 67 and 206 us where four take 55 and 103
 
 // Runs are as long as leaves `waves` waves (fewer rows are read twice); short sequences take shorter ones.
 ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int waves) {
@@ -258,23 +261,23 @@ ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int wav
   return s;
 }
 
-ConvShape fwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kFwdChannels, 16, 4, CONV_WF); }
-ConvShape bwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kBwdChannels, 64, 8, CONV_WB); }
+ConvShape fwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 16, 4, 8192); }
+ConvShape bwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 64, 8, 4096); }
 
 template <typename T>
 int conv_fwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {
-  if (K == 2) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 2, kFwdChannels>), grid, dim3(256), 0, s, a);
-  if (K == 3) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 3, kFwdChannels>), grid, dim3(256), 0, s, a);
-  if (K == 4) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 4, kFwdChannels>), grid, dim3(256), 0, s, a);
+  if (K == 2) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 2, kChannels>), grid, dim3(256), 0, s, a);
+  if (K == 3) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 3, kChannels>), grid, dim3(256), 0, s, a);
+  if (K == 4) hipLaunchKernelGGL((causal_conv_fwd_kernel<T, 4, kChannels>), grid, dim3(256), 0, s, a);
   SLAMHIP_HIP(hipGetLastError());
   return SLAMHIP_OK;
 }
 
 template <typename T>
 int conv_bwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {
-  if (K == 2) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 2, kBwdChannels>), grid, dim3(256), 0, s, a);
-  if (K == 3) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 3, kBwdChannels>), grid, dim3(256), 0, s, a);
-  if (K == 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 4, kBwdChannels>), grid, dim3(256), 0, s, a);
+  if (K == 2) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 2, kChannels>), grid, dim3(256), 0, s, a);
+  if (K == 3) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 3, kChannels>), grid, dim3(256), 0, s, a);
+  if (K == 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<T, 4, kChannels>), grid, dim3(256), 0, s, a);
   SLAMHIP_HIP(hipGetLastError());
   return SLAMHIP_OK;
 }

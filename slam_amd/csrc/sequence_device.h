@@ -27,19 +27,37 @@ struct Packed {
   typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
 
-// valid >= V: one vector access; fewer: element by element, the rest zero
+template <typename T, int V>
+using packed = typename Packed<T, V>::type;
+
+// valid >= V: one vector access; fewer (also none): element by element, the rest zero.  As they are in memory: a value that is
+// converted behind a condition is waited for there, one that is kept like this when it is used.
+template <int V, typename T>
+__device__ __forceinline__ packed<T, V> load_raw(const T* p, int valid) {
+  packed<T, V> raw;
+#pragma unroll
+  for (int i = 0; i < V; ++i) raw[i] = (T)0.0f;
+  if (valid >= V) {
+    raw = *reinterpret_cast<const packed<T, V>*>(p);
+  } else if (valid > 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < valid) raw[i] = p[i];
+  }
+  return raw;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ floats<V> to_floats(packed<T, V> raw) {
+  floats<V> v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = (float)raw[i];
+  return v;
+}
+
 template <int V, typename T>
 __device__ __forceinline__ floats<V> loadv(const T* p, int valid) {
-  floats<V> v;
-  if (valid >= V) {
-    const typename Packed<T, V>::type raw = *reinterpret_cast<const typename Packed<T, V>::type*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (float)raw[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = i < valid ? (float)p[i] : 0.0f;
-  }
-  return v;
+  return to_floats<T, V>(load_raw<V>(p, valid));
 }
 
 template <int V, typename T>

@@ -53,15 +53,18 @@ def _matrix(t, what):
     return t.shape[0], t.shape[1], _DTYPE[t.dtype], t.get_device()
 
 
-def _seq(t, dtype, shape, device, what, out=False):
-    """A sequence [B, T, C] of this type with unit stride over C; an output's rows may not overlap."""
+def _seq(t, dtype, shape, device, what, strides, out=False):
+    """The address of a sequence [B, T, C] of this type with unit stride over C; its strides over B and T join `strides`.  An
+    output's rows may not overlap."""
     if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != device:
         _bad(what, t, "a %s tensor %s on cuda:%d" % (dtype, shape, device))
-    (B, T, C), (sb, st, sc) = shape, t.stride()
+    sb, st, sc = t.stride()
+    B, T, C = shape
     if sc != 1 and C > 1:
         _bad(what, t, "unit stride over the last axis")
     if out and ((T > 1 and st < C) or (B > 1 and sb < C) or (B > 1 and T > 1 and sb < (T - 1) * st + C and st < (B - 1) * sb + C)):
         _bad(what, t, "rows that do not overlap")
+    strides += (sb, st)
     return t.data_ptr()
 
 
@@ -73,18 +76,14 @@ def _sequence(t, what):
     return B, T, C, t.dtype, t.get_device()
 
 
-def _strides(*ts):
-    v = []
-    for t in ts:
-        v += (0, 0) if t is None else t.stride()[:2]
-    return (ctypes.c_longlong * len(v))(*v)
+def _host_array(strides):
+    return (ctypes.c_longlong * len(strides))(*strides)
 
 
 def _apart(outs, ins):
-    """No output begins where an input does: runs of a sequence are worked on at once."""
-    taken = {t.data_ptr() for t in ins if t is not None and t.numel()}
-    for t in outs:
-        if t is not None and t.numel() and t.data_ptr() in taken:
+    """No output begins where an input does (addresses; 0 and None are no memory): steps of a sequence are worked on at once."""
+    for o in outs:
+        if o and o in ins:
             raise ValueError("an output is one of the inputs")
 
 
@@ -155,13 +154,15 @@ def causal_conv_fwd(x, weight, bias, y, state_in=None, state_out=None, lengths=N
     continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths (int32 [B]) bounds each sequence:
     rows behind it are not used and are zero in y.  x and y may be views with any strides over B and T."""
     B, T, C, dt, dev = _sequence(x, "x")
-    _seq(x, dt, (B, T, C), dev, "x")
+    strides = []
+    xp = _seq(x, dt, (B, T, C), dev, "x", strides)
+    yp = _seq(y, dt, (B, T, C), dev, "y", strides, out=True)
     w, K = _taps(weight, C, dev)
-    _apart((y, state_out), (x,))
-    _apart((y,), (state_in,))
-    _launch(dev, "slamhip_causal_conv_fwd", x.data_ptr(), _strides(x, y), w, _opt(bias, F32, (C,), dev, "bias"),
-            _opt(state_in, dt, (B, K - 1, C), dev, "state_in"), _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K,
-            int(silu), _DTYPE[dt], _seq(y, dt, (B, T, C), dev, "y", out=True), _opt(state_out, dt, (B, K - 1, C), dev, "state_out"))
+    sp, op = _opt(state_in, dt, (B, K - 1, C), dev, "state_in"), _opt(state_out, dt, (B, K - 1, C), dev, "state_out")
+    _apart((yp, op), (xp,))
+    _apart((yp,), (sp, op))
+    _launch(dev, "slamhip_causal_conv_fwd", xp, _host_array(strides), w, _opt(bias, F32, (C,), dev, "bias"), sp,
+            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K, int(silu), _DTYPE[dt], yp, op)
 
 
 def causal_conv_bwd(dy, x, weight, bias, dx, dweight, dbias=None, state_in=None, d_state_in=None, d_state_out=None, lengths=None,
@@ -169,17 +170,19 @@ def causal_conv_bwd(dy, x, weight, bias, dx, dweight, dbias=None, state_in=None,
     """Gradients of causal_conv_fwd (same x, weight, bias, state_in, lengths, silu): dx, dweight, dbias and d_state_in from dy
     and from d_state_out, the gradient that arrives at state_out."""
     B, T, C, dt, dev = _sequence(x, "x")
-    _seq(x, dt, (B, T, C), dev, "x")
+    strides = []
+    yp = _seq(dy, dt, (B, T, C), dev, "dy", strides)
+    xp = _seq(x, dt, (B, T, C), dev, "x", strides)
+    dp = _seq(dx, dt, (B, T, C), dev, "dx", strides, out=True)
     w, K = _taps(weight, C, dev)
-    _apart((dx, d_state_in), (dy, x, state_in, d_state_out))
-    lib = capi.load()
-    nbytes = lib.slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K)
+    ip, op = _opt(state_in, dt, (B, K - 1, C), dev, "state_in"), _opt(d_state_out, dt, (B, K - 1, C), dev, "d_state_out")
+    gp = _opt(d_state_in, dt, (B, K - 1, C), dev, "d_state_in")
+    _apart((dp, gp), (yp, xp, ip, op))
+    nbytes = capi.load().slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, "slamhip_causal_conv_bwd", _seq(dy, dt, (B, T, C), dev, "dy"), x.data_ptr(), _strides(dy, x, dx), w,
-            _opt(bias, F32, (C,), dev, "bias"), _opt(state_in, dt, (B, K - 1, C), dev, "state_in"),
-            _opt(d_state_out, dt, (B, K - 1, C), dev, "d_state_out"), _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K,
-            int(silu), _DTYPE[dt], _seq(dx, dt, (B, T, C), dev, "dx", out=True), _flat(dweight, F32, (C, K), dev, "dweight"),
-            _opt(dbias, F32, (C,), dev, "dbias"), _opt(d_state_in, dt, (B, K - 1, C), dev, "d_state_in"), ws.data_ptr(), nbytes)
+    _launch(dev, "slamhip_causal_conv_bwd", yp, xp, _host_array(strides), w, _opt(bias, F32, (C,), dev, "bias"), ip, op,
+            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K, int(silu), _DTYPE[dt], dp,
+            _flat(dweight, F32, (C, K), dev, "dweight"), _opt(dbias, F32, (C,), dev, "dbias"), gp, ws.data_ptr(), nbytes)
 
 
 def selective_scan_kept_states(B, T, C, N, device):
@@ -187,15 +190,18 @@ def selective_scan_kept_states(B, T, C, N, device):
     return torch.empty(capi.load().slamhip_selective_scan_kept_floats(B, T, C, N), dtype=F32, device=device)
 
 
-def _scan_inputs(u, delta, A, Bm, Cm, z):
+def _scan_inputs(u, delta, A, Bm, Cm, z, strides):
     B, T, C, dt, dev = _sequence(u, "u")
     if A.dim() != 2 or not 1 <= A.shape[1] <= 32:
         _bad("A", A, "[%d, N] with 1 <= N <= 32" % C)
     N = A.shape[1]
-    ptrs = (_seq(u, dt, (B, T, C), dev, "u"), _seq(delta, dt, (B, T, C), dev, "delta"),
-            None if z is None else _seq(z, dt, (B, T, C), dev, "z"), _seq(Bm, dt, (B, T, N), dev, "Bm"),
-            _seq(Cm, dt, (B, T, N), dev, "Cm"))
-    return B, T, C, N, dt, dev, ptrs
+    up, dp = _seq(u, dt, (B, T, C), dev, "u", strides), _seq(delta, dt, (B, T, C), dev, "delta", strides)
+    zp = None
+    if z is None:
+        strides += (0, 0)
+    else:
+        zp = _seq(z, dt, (B, T, C), dev, "z", strides)
+    return B, T, C, N, dt, dev, (up, dp, zp, _seq(Bm, dt, (B, T, N), dev, "Bm", strides), _seq(Cm, dt, (B, T, N), dev, "Cm", strides))
 
 
 def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, softplus=True, state_in=None, state_out=None,
@@ -206,37 +212,44 @@ def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, 
     to be state_in of the call that continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths
     (int32 [B]) bounds each sequence: rows behind it are not used and are zero in y.  kept_states (selective_scan_kept_states)
     is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T."""
-    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z)
-    _apart((y,), (u, delta, z, Bm, Cm))
+    strides = []
+    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z, strides)
+    yp = _seq(y, dt, (B, T, C), dev, "y", strides, out=True)
+    _apart((yp,), ptrs)
     lib = capi.load()
+    kp = ws = None
     if kept_states is not None:
-        _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
+        kp = _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
     nbytes = lib.slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch(dev, "slamhip_selective_scan_fwd", *ptrs, _strides(u, delta, z, Bm, Cm, y), _flat(A, F32, (C, N), dev, "A"),
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "slamhip_selective_scan_fwd", *ptrs, _host_array(strides), _flat(A, F32, (C, N), dev, "A"),
             _opt(D, F32, (C,), dev, "D"), _opt(delta_bias, F32, (C,), dev, "delta_bias"), _opt(state_in, F32, (B, C, N), dev, "state_in"),
-            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt],
-            _seq(y, dt, (B, T, C), dev, "y", out=True), _opt(state_out, F32, (B, C, N), dev, "state_out"), capi.ptr(kept_states),
-            capi.ptr(ws), nbytes)
+            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt], yp,
+            _opt(state_out, F32, (B, C, N), dev, "state_out"), kp, capi.ptr(ws), nbytes)
 
 
 def selective_scan_bwd(dy, u, delta, A, Bm, Cm, kept_states, du, ddelta, dA, dB, dC, D=None, z=None, delta_bias=None, softplus=True,
                        dD=None, dz=None, d_delta_bias=None, d_state_in=None, d_state_out=None, lengths=None):
     """Gradients of selective_scan_fwd at the same inputs, with the states that it kept, from dy and from d_state_out, the
     gradient that arrives at state_out: du, ddelta, dz (given when z is), dB, dC, dA, dD, d_delta_bias and d_state_in."""
-    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z)
-    outs = tuple(None if t is None else _seq(t, dt, (B, T, w), dev, what, out=True) for t, w, what in
-                 ((du, C, "du"), (ddelta, C, "ddelta"), (dz, C, "dz"), (dB, N, "dB"), (dC, N, "dC")))
-    if (z is None) != (dz is None) or du is None or ddelta is None or dB is None or dC is None:
-        raise ValueError("selective_scan_bwd: du, ddelta, dB, dC are wanted, and dz exactly when there is z")
-    _apart((du, ddelta, dz, dB, dC, d_state_in), (dy, u, delta, z, Bm, Cm, d_state_out))
+    if (z is None) != (dz is None):
+        raise ValueError("selective_scan_bwd: dz is wanted exactly when there is z")
+    strides, out_strides = [], []
+    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z, strides)
+    outs = [_seq(t, dt, (B, T, w), dev, what, out_strides, out=True) for t, w, what in
+            ((du, C, "du"), (ddelta, C, "ddelta"), (u if dz is None else dz, C, "dz"), (dB, N, "dB"), (dC, N, "dC"))]
+    if dz is None:
+        outs[2] = None
+    yp = _seq(dy, dt, (B, T, C), dev, "dy", out_strides)
+    gp, op = _opt(d_state_in, F32, (B, C, N), dev, "d_state_in"), _opt(d_state_out, F32, (B, C, N), dev, "d_state_out")
+    _apart((*outs, gp), (*ptrs, yp, op))
     lib = capi.load()
-    _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
+    kp = _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
     nbytes = lib.slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, "slamhip_selective_scan_bwd", _seq(dy, dt, (B, T, C), dev, "dy"), *ptrs,
-            _strides(dy, u, delta, z, Bm, Cm, du, ddelta, dz, dB, dC), _flat(A, F32, (C, N), dev, "A"), _opt(D, F32, (C,), dev, "D"),
-            _opt(delta_bias, F32, (C,), dev, "delta_bias"), kept_states.data_ptr(), _opt(d_state_out, F32, (B, C, N), dev, "d_state_out"),
+    _launch(dev, "slamhip_selective_scan_bwd", yp, *ptrs, _host_array(out_strides[10:] + strides + out_strides[:10]),
+            _flat(A, F32, (C, N), dev, "A"), _opt(D, F32, (C,), dev, "D"), _opt(delta_bias, F32, (C,), dev, "delta_bias"), kp, op,
             _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt], *outs,
             _flat(dA, F32, (C, N), dev, "dA"), _opt(dD, F32, (C,), dev, "dD"), _opt(d_delta_bias, F32, (C,), dev, "d_delta_bias"),
-            _opt(d_state_in, F32, (B, C, N), dev, "d_state_in"), ws.data_ptr(), nbytes)
+            gp, ws.data_ptr(), nbytes)

@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(256, 4) selective_scan_fwd_kernel(ScanArgs a) 
   } else if (chunk == 0) {
     load_states<P>(a.ends + ((long long)l.b * slots * a.C + l.cc) * a.N, a.N, l.q, h);
   } else {
+#pragma unroll 4
     for (int j = 0; j < chunk; ++j) {
       const float s = a.sums[((long long)l.b * a.chunks + j) * a.C + l.cc];
       float e[P];
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
   if (!CARRY || chunk == a.chunks - 1)
     if (a.d_state_out) load_states<P>(a.d_state_out + bC * a.N, a.N, l.q, g);
   if (!CARRY)
+#pragma unroll 4
     for (int j = a.chunks - 1; j > chunk; --j) {   // the last chunk's own carry holds d_state_out already
       const float s = a.sums[((long long)l.b * a.chunks + j) * a.C + l.cc];
       float e[P];
@@ -687,15 +689,20 @@ struct ScanShape {
 };
 
 // Chunks, where the channels alone give fewer waves than two a SIMD (2048): then as many as make eight (a first pass costs two
-// thirds of the second whatever their number), none of under 64 steps.  Measured at 8 x 2048 steps x 2048 channels x 16 states
-// (1024 waves): whole 271 us forward and 665 us back, cut in 8 98 + 180 us and 105 + 495 us.
+// thirds of the second whatever their number).  Measured at 8 x 2048 steps x 2048 channels x 16 states (1024 waves): whole 271 us
+// forward and 665 us back, cut in 8 98 + 180 us and 105 + 495 us; at 1024 waves and more a short sequence stays whole (32 x 130 x
+// 700 x 4 forward 22 us, cut 25 us).  A chunk also joins all those in front of it, one after the other, so none is shorter than
+// the square root of the sequence: 1 x 4096 x 64 x 16 forward takes 83, 48, 36, 41 us in chunks of 16, 32, 64, 128, and
+// 1 x 200 x 512 x 16 takes 12, 15, 21 us in chunks of 16, 32, 64.
 ScanShape scan_shape(int B, int T, int C, int N) {
   ScanShape s;
   s.P = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
   s.groups = (C + 63) / 64;
   const long long waves = (long long)B * s.groups * 4;
-  long long chunks = waves >= 2048 ? 1 : (8192 + waves - 1) / waves;
-  if (chunks > T / 64) chunks = T / 64;
+  int shortest = 16;
+  while ((long long)shortest * shortest < T) shortest += 16;
+  long long chunks = waves >= 2048 || (waves >= 1024 && T < 512) ? 1 : (8192 + waves - 1) / waves;
+  if (chunks > T / shortest) chunks = T / shortest;
   if (chunks < 1) chunks = 1;
   const int per = (int)((T + chunks - 1) / chunks);
   s.chunk = (per + 15) / 16 * 16;

@@ -113,7 +113,8 @@ SIGNATURES = {
     "slamhip_rms_norm_bwd": ([_c_void_p] * 5 + [ctypes.c_longlong, _c_int, _c_int] + [_c_void_p] * 3 + [ctypes.c_size_t, _c_void_p], _c_int),
     "slamhip_quantize_fp8": ([_c_void_p, ctypes.c_longlong, _c_int, _c_int] + [_c_void_p] * 3, _c_int),
     "slamhip_quantize_fp8_blocks": ([_c_void_p, _c_int, _c_int, _c_int] + [_c_void_p] * 3, _c_int),
-    "slamhip_gemm_nt_fp8": ([_c_void_p] * 4 + [_c_int] * 3 + [_c_void_p] * 2, _c_int),
+    "slamhip_gemm_nt_fp8_workspace_bytes": ([_c_int] * 3, ctypes.c_size_t),
+    "slamhip_gemm_nt_fp8": ([_c_void_p] * 4 + [_c_int] * 3 + [_c_void_p] * 2 + [ctypes.c_size_t, _c_void_p], _c_int),
     "slamhip_causal_conv_fwd": ([_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p] * 3, _c_int),
     "slamhip_causal_conv_bwd_workspace_bytes": ([_c_int] * 4, ctypes.c_size_t),
     "slamhip_causal_conv_bwd": ([_c_void_p] * 8 + [_c_int] * 6 + [_c_void_p] * 5 + [ctypes.c_size_t, _c_void_p], _c_int),

@@ -27,6 +27,8 @@ struct GemmArgs {
   const float *sa, *sb;
   __bf16* out;
   int M, N, K, KB;
+  int per;       // blocks of k a workgroup, a multiple of 4; workgroups (.., y) begin at block y * per
+  float* part;   // with more than one such part: their sums, float32 [parts][M][N]
 };
 
 __device__ __forceinline__ f32x4 mfma_fp8(i32x8 x, i32x8 y) {
@@ -43,6 +45,10 @@ typedef bf16x4 bf16x4_b __attribute__((aligned(2)));
 // four columns n .. n + 3 of row m
 __device__ __forceinline__ void store_out(const GemmArgs& p, int m, int n, f32x4 v) {
   if (m >= p.M || n >= p.N) return;
+  if (p.part) {
+    storev<4>(p.part + ((long long)blockIdx.y * p.M + m) * p.N + n, v, p.N - n);
+    return;
+  }
   __bf16* o = p.out + (long long)m * p.N + n;
   if (n + 4 <= p.N) {
     *reinterpret_cast<bf16x4_b*>(o) = __builtin_convertvector(v, bf16x4);
@@ -87,6 +93,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
   const int band = work / (8 * tiles_n), high = min(8, tiles_m - band * 8), in_band = work - band * 8 * tiles_n;
   const int m0 = (band * 8 + in_band % high) * BM, n0 = in_band / high * BN;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int kb_begin = blockIdx.y * p.per, kb_end = min(kb_begin + p.per, p.KB);
   const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, (unsigned)((size_t)p.M * p.K), 0x00020000);
   const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)p.b, 0, (unsigned)((size_t)p.N * p.K), 0x00020000);
   const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)p.sa, 0, (unsigned)((size_t)p.M * p.KB * 4), 0x00020000);
@@ -98,7 +105,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
   const unsigned off_b = (unsigned)(n0 + wave * 8 + lrow) * (unsigned)p.K + lchunk * 16;
   const unsigned off_s = (unsigned)(m0 + wave * 64 + lane) * (unsigned)p.KB * 4;
   auto load = [&](int it, int buf) {
-    const int kb = it * KW + kg;
+    const int kb = kb_begin + it * KW + kg;
     const bool in = kb * 128 + lchunk * 16 < p.K;
     const unsigned va = in ? off_a : kBeyond, vb = in ? off_b : kBeyond;
     uint8_t* to = sh + (buf * KW + kg) * kSlice;
@@ -126,8 +133,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{};
-  load_scales(0);
-  load_scales(1);
+  load_scales(kb_begin >> 2);
+  load_scales((kb_begin >> 2) + 1);
 #pragma unroll
   for (int i = 0; i < NS; ++i) load(i, i);
   wait_loads<(NS - 1) * kLoads>();
@@ -140,9 +147,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
   // block's first fragments are read (a column's as soon as its registers are free) the matrix unit has that row to work on.
   // The loop has no branch: behind the last block zeros are brought and not used.
   int buf = 0;
-  float sb_next = sbp[min(kg, p.KB - 1)];
-  for (int it = 0; it * KW < p.KB; ++it) {
-    const int kb = it * KW + kg, next_buf = buf + 1 == NS ? 0 : buf + 1;
+  float sb_next = sbp[min(kb_begin + kg, p.KB - 1)];
+  for (int it = 0; kb_begin + it * KW < kb_end; ++it) {
+    const int kb = kb_begin + it * KW + kg, next_buf = buf + 1 == NS ? 0 : buf + 1;
     const uint8_t* base = sh + (buf * KW + kg) * kSlice;
     const uint8_t* other = sh + (next_buf * KW + kg) * kSlice;
     const float sb = sb_next;
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
     float s[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i) s[i] = *reinterpret_cast<const float*>(scales + (kb >> 2 & 3) * kScales + (wm + i * 16 + frow) * 16 + (kb & 3) * 4) * sb;
-    if (KW > 1 && kb >= p.KB)   // the last round of a group that has no block left
+    if (KW > 1 && kb >= kb_end)   // the last round of a group that has no block left
 #pragma unroll
       for (int i = 0; i < TM; ++i) s[i] = 0.0f;
     f32x4 d[2][2];
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
 #pragma unroll
       for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[i][j]));
     // two fours ahead: before the last wait in front of their first use two slices are asked for, as many as may be under way then
-    if ((it * KW & 3) == 0) load_scales((it * KW >> 2) + 2);
+    if ((it * KW & 3) == 0) load_scales(((kb_begin + it * KW) >> 2) + 2);
     buf = next_buf;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is under way to shared memory when the workgroup ends
@@ -209,93 +216,109 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
     for (int j = 0; j < TN; ++j) store_out(p, m0 + wm + i * 16 + frow, n0 + wn + j * 16 + g * 4, acc[i][j]);
 }
 
-// Few rows: the weights are read once, straight into registers; a workgroup's waves take every eighth block of k for the same 16
-// columns and meet in shared memory.  U blocks are loaded at once: the whole of K = 4096 for up to 16 rows.
-template <int TM, int U>
+// Up to 16 rows: the weights are read once, straight into registers (one fragment serves all rows); a workgroup's waves take every
+// eighth block of k for the same 16 columns and meet in shared memory.  U blocks are under way at once, all of K = 4096.  Bound by
+// the weights' bytes: 4 x 8192 x 4096 takes 9.5 us, 3.5 TB/s.  From 17 rows on the tiles are faster (12 against 18 us at 32 rows).
 __global__ void __launch_bounds__(512) gemm_fp8_rows_kernel(GemmArgs p) {
-  constexpr int kWaves = 8;
-  __shared__ f32x4 sh[kWaves][TM][64];
+  constexpr int kWaves = 8, U = 4;
+  __shared__ f32x4 sh[kWaves][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n0 = blockIdx.x * 16, row = lane & 15, g = lane >> 4;
+  const int m = min(row, p.M - 1);   // rows beyond the last repeat it and are not stored
+  const uint8_t* a = p.a + (long long)m * p.K;
+  const float* sap = p.sa + (long long)m * p.KB;
   const uint8_t* b = p.b + (long long)min(n0 + row, p.N - 1) * p.K;
   ConstFloat* sbp = uniform_floats(p.sb + (long long)(n0 / 128) * p.KB);
-  const uint8_t* a[TM];
-  const float* sap[TM];
-  f32x4 acc[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = min(i * 16 + row, p.M - 1);   // rows beyond the last repeat it and are not stored
-    a[i] = p.a + (long long)m * p.K;
-    sap[i] = p.sa + (long long)m * p.KB;
-    acc[i] = f32x4{};
-  }
-  for (int kb0 = wave; kb0 < p.KB; kb0 += kWaves * U) {
-    i32x8 fb[U], fa[TM][U];
-    float sa[TM][U], sb[U];
+  f32x4 acc{};
+  const int kb_begin = blockIdx.y * p.per, kb_end = min(kb_begin + p.per, p.KB);
+  for (int kb0 = kb_begin + wave; kb0 < kb_end; kb0 += kWaves * U) {
+    i32x8 fb[U], fa[U];
+    float s[U];
     const i32x4 zero{};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int kb = kb0 + u * kWaves, k0 = kb * 128 + g * 16, k1 = k0 + 64;
-      const bool in0 = k0 < p.K, in1 = k1 < p.K;
+      const bool in0 = k0 < p.K && kb < kb_end, in1 = k1 < p.K && kb < kb_end;
       fb[u] = join(in0 ? *reinterpret_cast<const i32x4*>(b + k0) : zero, in1 ? *reinterpret_cast<const i32x4*>(b + k1) : zero);
-      sb[u] = kb < p.KB ? sbp[kb] : 0.0f;
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        fa[i][u] = join(in0 ? *reinterpret_cast<const i32x4*>(a[i] + k0) : zero, in1 ? *reinterpret_cast<const i32x4*>(a[i] + k1) : zero);
-        sa[i][u] = kb < p.KB ? sap[i][kb] : 0.0f;
-      }
+      fa[u] = join(in0 ? *reinterpret_cast<const i32x4*>(a + k0) : zero, in1 ? *reinterpret_cast<const i32x4*>(a + k1) : zero);
+      s[u] = kb < kb_end ? sap[kb] * sbp[kb] : 0.0f;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const f32x4 d = mfma_fp8(fb[u], fa[u]);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const f32x4 d = mfma_fp8(fb[u], fa[i][u]);
-        const float s = sa[i][u] * sb[u];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(d[r], s, acc[i][r]);
-      }
+      for (int r = 0; r < 4; ++r) acc[r] = fmaf(d[r], s[u], acc[r]);
+    }
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) sh[wave][i][lane] = acc[i];
+  sh[wave][lane] = acc;
   __syncthreads();
-  for (int i = wave; i < TM; i += kWaves) {
-    f32x4 v = sh[0][i][lane];
-    for (int w = 1; w < kWaves; ++w) v += sh[w][i][lane];
-    store_out(p, i * 16 + row, n0 + g * 4, v);
+  if (wave == 0) {
+    for (int w = 1; w < kWaves; ++w) acc += sh[w][lane];
+    store_out(p, row, n0 + g * 4, acc);
   }
 }
 
-template <int BM, int BN, int WM, int WN, int NS, int KW>
-int gemm_tiles(const GemmArgs& p, hipStream_t s) {
-  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  SLAMHIP_REQUIRE(tiles < (1 << 22), SLAMHIP_E_SIZE, "gemm_nt_fp8: too many tiles");
-  hipLaunchKernelGGL((gemm_fp8_kernel<BM, BN, WM, WN, NS, KW>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN * KW), 0, s, p);
-  SLAMHIP_HIP(hipGetLastError());
-  return SLAMHIP_OK;
+__global__ void __launch_bounds__(256) gemm_fp8_parts_kernel(const float* __restrict__ part, int parts, long long n, __bf16* __restrict__ out) {
+  const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  const int valid = (int)min(n - at, 4LL);
+  f32x4 v = loadv<4>(part + at, valid);
+  for (int i = 1; i < parts; ++i) v += loadv<4>(part + i * n + at, valid);
+  storev<4>(out + at, v, valid);
 }
 
-int gemm(const GemmArgs& p, hipStream_t s) {
-  if (p.M <= 64) {
-    const dim3 grid((p.N + 15) / 16);
-    if (p.M <= 16)
-      hipLaunchKernelGGL((gemm_fp8_rows_kernel<1, 4>), grid, dim3(512), 0, s, p);
-    else if (p.M <= 32)
-      hipLaunchKernelGGL((gemm_fp8_rows_kernel<2, 2>), grid, dim3(512), 0, s, p);
-    else
-      hipLaunchKernelGGL((gemm_fp8_rows_kernel<4, 1>), grid, dim3(512), 0, s, p);
-    SLAMHIP_HIP(hipGetLastError());
-    return SLAMHIP_OK;
-  }
+// How a product is cut: the kernel by the number of rows and tiles, and parts of k where that leaves most CUs idle.
+struct GemmPlan {
+  enum Kind { kRows, k256, k128, k128KW, k64x128KW, k64KW } kind;
+  long long groups;
+  int per, parts;
+};
+
+GemmPlan gemm_plan(int M, int N, int K) {
+  GemmPlan g;
+  auto tiles = [&](int bm, int bn) { return (long long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  auto pick = [&](GemmPlan::Kind kind, long long groups) { g.kind = kind, g.groups = groups; };
   // The largest tiles that still give most of the 256 CUs one.  Smaller ones read operands more often, larger ones leave CUs idle;
   // two groups of waves (KW = 2) where a CU has one workgroup.  us, 256^2 / 128^2 / 128^2 KW / 64 x 128 KW / 64^2 KW:
   // 4096x4096x4096 68/83/93/115/153, 2048x4096x4096 59/42/48/59/77, 1024x4096x4096 57/28/26/31/40, 777x2056x4096 54/25/22/16/21,
   // 1024x1024x4096 56/25/22/16/12.
-  auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  if (tiles(256, 256) >= 192) return gemm_tiles<256, 256, 2, 4, 2, 1>(p, s);
-  if (tiles(128, 128) > 256) return gemm_tiles<128, 128, 2, 2, 2, 1>(p, s);
-  if (tiles(128, 128) > 128) return gemm_tiles<128, 128, 2, 2, 2, 2>(p, s);
-  if (tiles(64, 128) > 128) return gemm_tiles<64, 128, 2, 2, 3, 2>(p, s);
-  return gemm_tiles<64, 64, 2, 2, 4, 2>(p, s);
+  if (M <= 16) pick(GemmPlan::kRows, (N + 15) / 16);
+  else if (tiles(256, 256) >= 192) pick(GemmPlan::k256, tiles(256, 256));
+  else if (tiles(128, 128) > 256) pick(GemmPlan::k128, tiles(128, 128));
+  else if (tiles(128, 128) > 128) pick(GemmPlan::k128KW, tiles(128, 128));
+  else if (tiles(64, 128) > 128) pick(GemmPlan::k64x128KW, tiles(64, 128));
+  else pick(GemmPlan::k64KW, tiles(64, 64));
+  const int KB = (K + 127) / 128, least = 32;   // blocks of k that are worth a part of their own, and a launch more
+  long long parts = 256 / g.groups;
+  if (parts > KB / least) parts = KB / least;
+  if (parts < 1) parts = 1;
+  g.per = (int)(((KB + parts - 1) / parts + 3) / 4 * 4);
+  g.parts = (KB + g.per - 1) / g.per;
+  return g;
+}
+
+template <int BM, int BN, int WM, int WN, int NS, int KW>
+void gemm_tiles(const GemmArgs& p, const GemmPlan& g, hipStream_t s) {
+  hipLaunchKernelGGL((gemm_fp8_kernel<BM, BN, WM, WN, NS, KW>), dim3((unsigned)((g.groups + 7) / 8 * 8), g.parts), dim3(64 * WM * WN * KW), 0, s, p);
+}
+
+int gemm(const GemmArgs& p, const GemmPlan& g, hipStream_t s) {
+  const dim3 rows((unsigned)g.groups, g.parts);
+  switch (g.kind) {
+    case GemmPlan::kRows: hipLaunchKernelGGL(gemm_fp8_rows_kernel, rows, dim3(512), 0, s, p); break;
+    case GemmPlan::k256: gemm_tiles<256, 256, 2, 4, 2, 1>(p, g, s); break;
+    case GemmPlan::k128: gemm_tiles<128, 128, 2, 2, 2, 1>(p, g, s); break;
+    case GemmPlan::k128KW: gemm_tiles<128, 128, 2, 2, 2, 2>(p, g, s); break;
+    case GemmPlan::k64x128KW: gemm_tiles<64, 128, 2, 2, 3, 2>(p, g, s); break;
+    case GemmPlan::k64KW: gemm_tiles<64, 64, 2, 2, 4, 2>(p, g, s); break;
+  }
+  SLAMHIP_HIP(hipGetLastError());
+  if (g.parts > 1) {
+    const long long n = (long long)p.M * p.N;
+    hipLaunchKernelGGL(gemm_fp8_parts_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, p.part, g.parts, n, p.out);
+    SLAMHIP_HIP(hipGetLastError());
+  }
+  return SLAMHIP_OK;
 }
 
 }  // namespace
@@ -305,16 +328,27 @@ using namespace slamhip;
 
 extern "C" {
 
+size_t slamhip_gemm_nt_fp8_workspace_bytes(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const GemmPlan g = gemm_plan(M, N, K);
+  return g.parts > 1 ? (size_t)g.parts * M * N * sizeof(float) : 0;
+}
+
 int slamhip_gemm_nt_fp8(const void* a, const float* a_scales, const void* b, const float* b_scales, int M, int N, int K, void* out,
-                        void* stream) {
+                        void* workspace, size_t workspace_bytes, void* stream) {
   SLAMHIP_REQUIRE(M >= 0 && N >= 0 && K > 0, SLAMHIP_E_ARG, "gemm_nt_fp8: need M, N >= 0 and K >= 1");
   SLAMHIP_REQUIRE(K % 16 == 0, SLAMHIP_E_SIZE, "gemm_nt_fp8: K must be a multiple of 16");
   SLAMHIP_REQUIRE((M + 256LL) * K < (1LL << 31) && (N + 256LL) * K < (1LL << 31), SLAMHIP_E_SIZE, "gemm_nt_fp8: an operand is larger than 2 GB");
   if (M == 0 || N == 0) return SLAMHIP_OK;
   SLAMHIP_REQUIRE(a && a_scales && b && b_scales && out, SLAMHIP_E_ARG, "gemm_nt_fp8: null pointer");
   SLAMHIP_REQUIRE(((uintptr_t)a & 15) == 0 && ((uintptr_t)b & 15) == 0, SLAMHIP_E_ARG, "gemm_nt_fp8: operands must be 16-byte aligned");
-  const GemmArgs p{(const uint8_t*)a, (const uint8_t*)b, a_scales, b_scales, (__bf16*)out, M, N, K, (K + 127) / 128};
-  return gemm(p, (hipStream_t)stream);
+  const GemmPlan g = gemm_plan(M, N, K);
+  SLAMHIP_REQUIRE(g.groups < (1 << 22), SLAMHIP_E_SIZE, "gemm_nt_fp8: too many tiles");
+  SLAMHIP_REQUIRE(g.parts == 1 || (workspace && workspace_bytes >= (size_t)g.parts * M * N * sizeof(float)), SLAMHIP_E_ARG,
+                  "gemm_nt_fp8: workspace too small");
+  const GemmArgs p{(const uint8_t*)a, (const uint8_t*)b, a_scales, b_scales, (__bf16*)out, M, N, K, (K + 127) / 128, g.per,
+                   g.parts > 1 ? (float*)workspace : nullptr};
+  return gemm(p, g, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -245,7 +245,8 @@ quantize_fp8_blocks_kernel(const T* __restrict__ x, int R, int C, uint8_t* __res
 
 constexpr int kMaxSlots = 1024;
 
-int norm_slots(long long rows) { return (int)(rows < kMaxSlots ? rows : kMaxSlots); }
+// up to four rows one slot takes them all and its part is dw: a second launch costs more than three rows one after the other
+int norm_slots(long long rows) { return rows <= 0 ? 0 : rows <= 4 ? 1 : (int)(rows < kMaxSlots ? rows : kMaxSlots); }
 
 template <typename T, int LANES, int ITER>
 int norm_fwd(const void* x, const void* residual, const float* w, float eps, long long rows, int C, void* sum_out, void* y, void* y8,
@@ -261,11 +262,12 @@ template <typename T, int LANES, int ITER>
 int norm_bwd(const void* dy, const void* sum, const float* w, const float* rstd, const void* d_sum, long long rows, int C, void* dx,
              float* dw, float* part, hipStream_t s) {
   const int slots = norm_slots(rows), per = 256 / LANES;
+  if (slots == 1) part = dw;
   if (slots > 0)
     hipLaunchKernelGGL((rms_norm_bwd_kernel<T, LANES, ITER>), dim3((slots + per - 1) / per), dim3(256), 0, s, (const T*)dy, (const T*)sum,
                        w, rstd, (const T*)d_sum, rows, C, slots, (T*)dx, part);
   SLAMHIP_HIP(hipGetLastError());
-  SLAMHIP_HIP(column_sums(part, slots, C, WeightGradient{dw}, s));
+  if (slots != 1) SLAMHIP_HIP(column_sums(part, slots, C, WeightGradient{dw}, s));
   return SLAMHIP_OK;
 }
 
@@ -308,7 +310,7 @@ int slamhip_rms_norm_fwd(const void* x, const void* residual, const float* weigh
 
 size_t slamhip_rms_norm_bwd_workspace_bytes(long long rows, int C) {
   if (rows <= 0 || C <= 0) return 0;
-  return (size_t)norm_slots(rows) * (size_t)C * sizeof(float);
+  return norm_slots(rows) == 1 ? 0 : (size_t)norm_slots(rows) * (size_t)C * sizeof(float);
 }
 
 int slamhip_rms_norm_bwd(const void* dy, const void* sum, const float* weight, const float* rstd, const void* d_sum, long long rows,
@@ -316,8 +318,9 @@ int slamhip_rms_norm_bwd(const void* dy, const void* sum, const float* weight, c
   SLAMHIP_REQUIRE(rows >= 0 && C > 0 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG,
                   "rms_norm_bwd: need rows >= 0, C >= 1 and a known type");
   SLAMHIP_REQUIRE(C <= kMaxNormC && rows <= kMaxGroups, SLAMHIP_E_SIZE, "rms_norm_bwd: at most %d columns and 2^24 - 1 rows", kMaxNormC);
-  SLAMHIP_REQUIRE(dweight && (rows == 0 || (dy && sum && weight && rstd && dx && workspace)), SLAMHIP_E_ARG, "rms_norm_bwd: null pointer");
-  SLAMHIP_REQUIRE(workspace_bytes >= slamhip_rms_norm_bwd_workspace_bytes(rows, C), SLAMHIP_E_ARG, "rms_norm_bwd: workspace too small");
+  SLAMHIP_REQUIRE(dweight && (rows == 0 || (dy && sum && weight && rstd && dx)), SLAMHIP_E_ARG, "rms_norm_bwd: null pointer");
+  const size_t need = slamhip_rms_norm_bwd_workspace_bytes(rows, C);
+  SLAMHIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0), SLAMHIP_E_ARG, "rms_norm_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   SLAMHIP_NORM_DISPATCH(norm_bwd, dy, sum, weight, rstd, d_sum, rows, C, dx, dweight, (float*)workspace, s);
 }

@@ -651,38 +651,46 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
   }
 }
 
-// dB and dC from the parts of the channel groups; a thread a value
+// The parts of dB and dC (of the channel groups; a thread a value) and those of dA, dD and the bias (of sequences and chunks; 32
+// columns a workgroup), in one launch: the first bc_groups workgroups take dB and dC.  Fixed orders.
 template <typename T>
-__global__ void __launch_bounds__(256) selective_scan_bc_kernel(const float* __restrict__ part, int groups, int np, int N, long long steps,
-                                                                int T_, const int* __restrict__ lengths, T* dB, T* dC, long long dBb,
-                                                                long long dBt, long long dCb, long long dCt) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long step = at / (2 * np);
-  if (step >= steps) return;
-  const int v = (int)(at - step * 2 * np), which = v / np, n = v - which * np;
-  if (n >= N) return;
-  const int b = (int)(step / T_), t = (int)(step - (long long)b * T_);
-  float s = 0.0f;
-  for (int g = 0; g < groups; ++g) s += part[(step * groups + g) * 2 * np + v];
-  if (lengths && t >= lengths[b]) s = 0.0f;
-  if (which)
-    dC[b * dCb + t * dCt + n] = (T)s;
-  else
-    dB[b * dBb + t * dBt + n] = (T)s;
-}
-
-struct ScanGradients {
-  float *dA, *dD, *dbias;
-  int C, N;
-  __device__ void operator()(int i, float v) const {
-    if (i < C * N)
-      dA[i] = v;
-    else if (i < C * (N + 1)) {
-      if (dD) dD[i - C * N] = v;
-    } else if (dbias)
-      dbias[i - C * (N + 1)] = v;
+__global__ void __launch_bounds__(256) selective_scan_parts_kernel(ScanArgs a, int bc_groups, int groups, int np, int B, void* dB, void* dC,
+                                                                   long long dBb, long long dBt, long long dCb, long long dCt, float* dA,
+                                                                   float* dD, float* dbias) {
+  if ((int)blockIdx.x < bc_groups) {
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long step = at / (2 * np);
+    if (step >= (long long)B * a.T) return;
+    const int v = (int)(at - step * 2 * np), which = v / np, n = v - which * np;
+    if (n >= a.N) return;
+    const int b = (int)(step / a.T), t = (int)(step - (long long)b * a.T);
+    float s = 0.0f;
+    for (int g = 0; g < groups; ++g) s += a.part_bc[(step * groups + g) * 2 * np + v];
+    if (a.lengths && t >= a.lengths[b]) s = 0.0f;
+    if (which)
+      ((T*)dC)[b * dCb + t * dCt + n] = (T)s;
+    else
+      ((T*)dB)[b * dBb + t * dBt + n] = (T)s;
+    return;
   }
-};
+  __shared__ float sh[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, columns = a.C * (a.N + 2);
+  const int c = (blockIdx.x - bc_groups) * 32 + tx, parts = B * a.chunks;
+  float s = 0.0f;
+  if (c < columns)
+    for (int p = ty; p < parts; p += 8) s += a.part[(long long)p * columns + c];
+  sh[ty][tx] = s;
+  __syncthreads();
+  if (ty || c >= columns) return;
+  s = 0.0f;
+  for (int i = 0; i < 8; ++i) s += sh[i][tx];
+  if (c < a.C * a.N)
+    dA[c] = s;
+  else if (c < a.C * (a.N + 1)) {
+    if (dD) dD[c - a.C * a.N] = s;
+  } else if (dbias)
+    dbias[c - a.C * (a.N + 1)] = s;
+}
 
 struct ScanShape {
   int P, groups, chunk, chunks;
@@ -824,34 +832,34 @@ int slamhip_selective_scan_bwd(const void* dy, const void* u, const void* delta,
   SLAMHIP_REQUIRE(workspace_bytes >= slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N), SLAMHIP_E_ARG, "selective_scan_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const ScanShape g = scan_shape(B, T, C, N);
-  float* part = (float*)workspace;
-  SLAMHIP_REQUIRE((long long)C * (N + 2) <= 0x7fffffffLL, SLAMHIP_E_SIZE, "selective_scan_bwd: too many parameters");
+  const long long columns = (long long)C * (N + 2), bc_groups = work ? ((long long)B * T * 8 * g.P + 255) / 256 : 0;
+  const long long all_groups = bc_groups + (columns + 31) / 32;
+  SLAMHIP_REQUIRE(all_groups < (1 << 24) && (long long)B * g.chunks < (1 << 30), SLAMHIP_E_SIZE, "selective_scan_bwd: too many steps or parameters");
+  ScanArgs a{};
+  a.T = T, a.C = C, a.N = N, a.chunk = g.chunk, a.chunks = g.chunks, a.softplus = softplus, a.lengths = lengths;
+  a.part = (float*)workspace;
   if (work) {
-    ScanArgs a{};
     a.u = u, a.delta = delta, a.z = z, a.Bm = Bm, a.Cm = Cm, a.dy = dy, a.A = A, a.D = D, a.bias = delta_bias;
-    a.d_state_out = d_state_out, a.kept = const_cast<float*>(kept_states), a.lengths = lengths;
+    a.d_state_out = d_state_out, a.kept = const_cast<float*>(kept_states);
     a.du = du, a.ddelta = ddelta, a.dz = dz, a.d_state_in = d_state_in;
     a.dyb = strides[0], a.dyt = strides[1], a.ub = strides[2], a.ut = strides[3], a.deltab = strides[4], a.deltat = strides[5];
     a.zb = strides[6], a.zt = strides[7], a.Bb = strides[8], a.Bt = strides[9], a.Cb = strides[10], a.Ct = strides[11];
     a.dub = strides[12], a.dut = strides[13], a.ddeltab = strides[14], a.ddeltat = strides[15], a.dzb = strides[16], a.dzt = strides[17];
-    a.T = T, a.C = C, a.N = N, a.chunk = g.chunk, a.chunks = g.chunks, a.softplus = softplus;
-    a.part = part;
-    a.part_bc = part + (size_t)B * g.chunks * C * (N + 2);
+    a.part_bc = a.part + (size_t)B * g.chunks * columns;
     a.ends = a.part_bc + (size_t)B * T * g.groups * 8 * g.P;
     a.sums = a.ends + (size_t)B * g.chunks * C * N;
     const int rc = SLAMHIP_SCAN_DISPATCH(scan_bwd, g.P, a, g.groups, B, s);
     if (rc != SLAMHIP_OK) return rc;
-    const long long values = (long long)B * T * 8 * g.P, blocks = (values + 255) / 256;
-    SLAMHIP_REQUIRE(blocks < (1 << 24), SLAMHIP_E_SIZE, "selective_scan_bwd: too many steps");
-    if (dtype == SLAMHIP_BF16)
-      hipLaunchKernelGGL((selective_scan_bc_kernel<__bf16>), dim3((unsigned)blocks), dim3(256), 0, s, a.part_bc, g.groups, 4 * g.P, N,
-                         (long long)B * T, T, lengths, (__bf16*)dB, (__bf16*)dC, strides[18], strides[19], strides[20], strides[21]);
-    else
-      hipLaunchKernelGGL((selective_scan_bc_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, s, a.part_bc, g.groups, 4 * g.P, N,
-                         (long long)B * T, T, lengths, (float*)dB, (float*)dC, strides[18], strides[19], strides[20], strides[21]);
-    SLAMHIP_HIP(hipGetLastError());
   }
-  SLAMHIP_HIP(column_sums(part, work ? (long long)B * g.chunks : 0, C * (N + 2), ScanGradients{dA, dD, d_delta_bias, C, N}, s));
+  const long long none[4] = {0, 0, 0, 0}, *bc = work ? strides + 18 : none;
+  const int parts_of = work ? B : 0;   // nothing to add: the parameters' gradients are zero
+  if (dtype == SLAMHIP_BF16)
+    hipLaunchKernelGGL((selective_scan_parts_kernel<__bf16>), dim3((unsigned)all_groups), dim3(256), 0, s, a, (int)bc_groups, g.groups,
+                       4 * g.P, parts_of, dB, dC, bc[0], bc[1], bc[2], bc[3], dA, dD, d_delta_bias);
+  else
+    hipLaunchKernelGGL((selective_scan_parts_kernel<float>), dim3((unsigned)all_groups), dim3(256), 0, s, a, (int)bc_groups, g.groups,
+                       4 * g.P, parts_of, dB, dC, bc[0], bc[1], bc[2], bc[3], dA, dD, d_delta_bias);
+  SLAMHIP_HIP(hipGetLastError());
   return SLAMHIP_OK;
 }
 

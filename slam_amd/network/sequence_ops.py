@@ -136,9 +136,11 @@ def gemm_nt_fp8(a8, a_scales, b8, b_scales, out):
     kb = (K + 127) // 128
     if K % 16 or a8.data_ptr() % 16 or b8.data_ptr() % 16:
         raise ValueError("gemm_nt_fp8: K must be a multiple of 16 and the operands 16-byte aligned, got K = %d" % K)
+    nbytes = capi.load().slamhip_gemm_nt_fp8_workspace_bytes(M, N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch(dev, "slamhip_gemm_nt_fp8", _flat(a8, FP8, (M, K), dev, "a8"), _flat(a_scales, F32, (M, kb), dev, "a_scales"),
             _flat(b8, FP8, (N, K), dev, "b8"), _flat(b_scales, F32, ((N + 127) // 128, kb), dev, "b_scales"), M, N, K,
-            _flat(out, BF16, (M, N), dev, "out"))
+            _flat(out, BF16, (M, N), dev, "out"), capi.ptr(ws), nbytes)
 
 
 def _taps(weight, C, device):

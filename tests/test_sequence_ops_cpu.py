@@ -46,12 +46,16 @@ def test_quantize_and_product_refusals():
     refused(E_SIZE, "rows", "slamhip_quantize_fp8_blocks", P, 65535 * 128 + 1, 128, F32, P, P, None)
     refused(E_ARG, "null", "slamhip_quantize_fp8_blocks", P, 1, 8, F32, P, None, None)
     g = "slamhip_gemm_nt_fp8"
-    refused(E_ARG, "K >= 1", g, P, P, P, P, 1, 1, 0, P, None)
-    refused(E_SIZE, "multiple of 16", g, P, P, P, P, 1, 1, 24, P, None)
-    refused(E_SIZE, "2 GB", g, P, P, P, P, 1 << 20, 1, 4096, P, None)
-    refused(E_ARG, "null", g, P, None, P, P, 1, 1, 16, P, None)
-    refused(E_ARG, "aligned", g, ctypes.c_void_p(4104), P, P, P, 1, 1, 16, P, None)
-    assert capi.load().slamhip_gemm_nt_fp8(None, None, None, None, 0, 8, 16, None, None) == 0
+    refused(E_ARG, "K >= 1", g, P, P, P, P, 1, 1, 0, P, None, 0, None)
+    refused(E_SIZE, "multiple of 16", g, P, P, P, P, 1, 1, 24, P, None, 0, None)
+    refused(E_SIZE, "2 GB", g, P, P, P, P, 1 << 20, 1, 4096, P, None, 0, None)
+    refused(E_ARG, "null", g, P, None, P, P, 1, 1, 16, P, None, 0, None)
+    refused(E_ARG, "aligned", g, ctypes.c_void_p(4104), P, P, P, 1, 1, 16, P, None, 0, None)
+    need = capi.load().slamhip_gemm_nt_fp8_workspace_bytes(100, 64, 8192)      # two tiles: cut along k
+    assert need > 0 and capi.load().slamhip_gemm_nt_fp8_workspace_bytes(8192, 8192, 4096) == 0
+    refused(E_ARG, "workspace", g, P, P, P, P, 100, 64, 8192, P, P, need - 1, None)
+    refused(E_ARG, "workspace", g, P, P, P, P, 100, 64, 8192, P, None, need, None)
+    assert capi.load().slamhip_gemm_nt_fp8(None, None, None, None, 0, 8, 16, None, None, 0, None) == 0
 
 
 def test_causal_conv_refusals():

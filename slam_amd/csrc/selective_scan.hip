@@ -706,7 +706,7 @@ ScanShape scan_shape(int B, int T, int C, int N) {
   ScanShape s;
   s.P = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
   s.groups = (C + 63) / 64;
-  const long long waves = (long long)B * s.groups * 4;
+  const long long waves = (long long)(B > 0 ? B : 1) * s.groups * 4;   // without sequences the parameters' gradients are still asked for
   int shortest = 16;
   while ((long long)shortest * shortest < T) shortest += 16;
   long long chunks = waves >= 2048 || (waves >= 1024 && T < 512) ? 1 : (8192 + waves - 1) / waves;
@@ -806,13 +806,15 @@ int slamhip_selective_scan_fwd(const void* u, const void* delta, const void* z, 
   a.ub = strides[0], a.ut = strides[1], a.deltab = strides[2], a.deltat = strides[3], a.zb = strides[4], a.zt = strides[5];
   a.Bb = strides[6], a.Bt = strides[7], a.Cb = strides[8], a.Ct = strides[9], a.yb = strides[10], a.yt = strides[11];
   a.T = T, a.C = C, a.N = N, a.chunk = g.chunk, a.chunks = g.chunks, a.softplus = softplus;
-  a.ends = (float*)workspace;
-  a.sums = a.ends + (size_t)B * (g.chunks + 1) * C * N;
+  if (g.chunks > 1) {
+    a.ends = (float*)workspace;
+    a.sums = a.ends + (size_t)B * (g.chunks + 1) * C * N;
+  }
   return SLAMHIP_SCAN_DISPATCH(scan_fwd, g.P, a, g.groups, B, (hipStream_t)stream);
 }
 
 size_t slamhip_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N) {
-  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  if (B <= 0 || T < 0 || C <= 0 || N <= 0 || N > 32) return 0;
   const ScanShape g = scan_shape(B, T, C, N);
   const size_t carry = g.chunks > 1 ? (size_t)B * g.chunks * C * (N + 1) : 0;
   return (carry + (size_t)B * g.chunks * C * (N + 2) + (size_t)B * T * g.groups * 8 * g.P) * sizeof(float);
@@ -824,11 +826,11 @@ int slamhip_selective_scan_bwd(const void* dy, const void* u, const void* delta,
                                int softplus, int dtype, void* du, void* ddelta, void* dz, void* dB, void* dC, float* dA, float* dD,
                                float* d_delta_bias, float* d_state_in, void* workspace, size_t workspace_bytes, void* stream) {
   SLAMHIP_SCAN_SIZES("selective_scan_bwd");
-  const bool work = B > 0 && T > 0;
-  SLAMHIP_REQUIRE(dA && (!work || (A && strides && dy && u && delta && Bm && Cm && kept_states && du && ddelta && dB && dC && workspace)),
+  const bool work = B > 0, data = work && T > 0;
+  SLAMHIP_REQUIRE(dA && (!work || (A && strides && workspace)) &&
+                      (!data || (dy && u && delta && Bm && Cm && kept_states && du && ddelta && dB && dC)),
                   SLAMHIP_E_ARG, "selective_scan_bwd: null pointer");
-  SLAMHIP_REQUIRE(!work || !z == !dz, SLAMHIP_E_ARG, "selective_scan_bwd: z and dz come together");
-  SLAMHIP_REQUIRE(work || B == 0 || !d_state_in, SLAMHIP_E_ARG, "selective_scan_bwd: no steps");
+  SLAMHIP_REQUIRE(!data || !z == !dz, SLAMHIP_E_ARG, "selective_scan_bwd: z and dz come together");
   SLAMHIP_REQUIRE(workspace_bytes >= slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N), SLAMHIP_E_ARG, "selective_scan_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const ScanShape g = scan_shape(B, T, C, N);

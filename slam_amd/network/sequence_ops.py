@@ -5,7 +5,9 @@ norm, 8-bit operands and their product, short causal convolution, selective scan
 As in encoder_ops the caller brings GPU tensors for inputs and outputs, every call is
 checked on the host and launches on the current stream (of the tensors' device), and
 there is no autograd: a backward pass is a call of its own.  A refused call raises
-ValueError and launches nothing.  Activations are float32 or bfloat16, parameters,
+ValueError (what the tensors show) or RuntimeError (the library's limits of sizes and
+combinations) and launches nothing.  Outputs share no memory with each other or with
+inputs where a call does not say so.  Activations are float32 or bfloat16, parameters,
 statistics and states float32.  Workspaces are torch allocations of the call.
 """
 import ctypes
@@ -81,10 +83,14 @@ def _host_array(strides):
 
 
 def _apart(outs, ins):
-    """No output begins where an input does (addresses; 0 and None are no memory): steps of a sequence are worked on at once."""
+    """No output begins where an input or another output does (addresses; 0 and None are no memory): steps of a sequence are
+    worked on at once."""
+    seen = list(ins)
     for o in outs:
-        if o and o in ins:
-            raise ValueError("an output is one of the inputs")
+        if o:
+            if o in seen:
+                raise ValueError("an output is one of the inputs or another output")
+            seen.append(o)
 
 
 def rms_norm_fwd(x, weight, eps, y=None, residual=None, sum_out=None, y8=None, scales=None, rstd=None):
@@ -239,10 +245,13 @@ def selective_scan_bwd(dy, u, delta, A, Bm, Cm, kept_states, du, ddelta, dA, dB,
         raise ValueError("selective_scan_bwd: dz is wanted exactly when there is z")
     strides, out_strides = [], []
     B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z, strides)
-    outs = [_seq(t, dt, (B, T, w), dev, what, out_strides, out=True) for t, w, what in
-            ((du, C, "du"), (ddelta, C, "ddelta"), (u if dz is None else dz, C, "dz"), (dB, N, "dB"), (dC, N, "dC"))]
-    if dz is None:
-        outs[2] = None
+    outs = []
+    for t, w, what in ((du, C, "du"), (ddelta, C, "ddelta"), (dz, C, "dz"), (dB, N, "dB"), (dC, N, "dC")):
+        if t is None and what == "dz":
+            outs.append(None)
+            out_strides += (0, 0)
+        else:
+            outs.append(_seq(t, dt, (B, T, w), dev, what, out_strides, out=True))
     yp = _seq(dy, dt, (B, T, C), dev, "dy", out_strides)
     gp, op = _opt(d_state_in, F32, (B, C, N), dev, "d_state_in"), _opt(d_state_out, F32, (B, C, N), dev, "d_state_out")
     _apart((*outs, gp), (*ptrs, yp, op))

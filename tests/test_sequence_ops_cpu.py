@@ -137,3 +137,13 @@ def test_restatement_rounds_to_e4m3_like_torch():
     v = torch.cat((torch.linspace(-500, 500, 4001, dtype=torch.float64), torch.logspace(-5, 0, 2001, dtype=torch.float64)))
     want = v.float().clamp(-448, 448).to(torch.float8_e4m3fn).double()
     assert torch.equal(so.round_e4m3(v.float().double()), want)
+
+
+def test_workspaces_of_empty_calls():
+    """No sequences or no steps."""
+    lib = capi.load()
+    for B, T in ((0, 0), (0, 7), (3, 0)):
+        assert lib.slamhip_selective_scan_kept_floats(B, T, 5, 16) == 0
+        assert lib.slamhip_selective_scan_fwd_workspace_bytes(B, T, 5, 16) == 0
+        # the state's gradient passes through and the parameters' are zero: a sum for each sequence
+        assert lib.slamhip_selective_scan_bwd_workspace_bytes(B, T, 5, 16) == (0 if B == 0 else B * 5 * 18 * 4)

@@ -164,7 +164,9 @@ def test_quantize_special_values():
 GEMM_SHAPES = [(1, 1, 16), (1, 16, 128), (3, 130, 272), (16, 64, 4096), (17, 48, 640), (33, 200, 144), (64, 16, 128), (65, 1, 16), (65, 129, 400),
                (128, 128, 128), (200, 300, 1040), (257, 513, 384), (300, 64, 2048), (777, 520, 1024),
                # one for each tile shape, with odd edges: 64 x 128, 128 x 128 in two groups and in one, 256 x 256; 3, 5 and 9 blocks of k
-               (700, 1500, 384), (1500, 1400, 272), (2100, 2050, 640), (3500, 3400, 1152)]
+               (700, 1500, 384), (1500, 1400, 272), (2100, 2050, 640), (3500, 3400, 1152),
+               # few tiles and much k: parts of k, of which the last is short
+               (5, 40, 8336), (100, 70, 9232), (300, 200, 12304)]
 
 
 def gemm_bound(av, bv):
@@ -441,13 +443,401 @@ def test_empty_sequences(T):
     ops.causal_conv_bwd(z(B, T, C), z(B, T, C), torch.ones(C, K, device=DEV), None, y, dw, state_in=rows, d_state_in=din, d_state_out=left,
                         lengths=lengths)
     assert torch.equal(din, left) and not bool(dw.any())
+    # the scan back: the gradient of the state passes through, nothing else gets any
+    kept = ops.selective_scan_kept_states(B, T, C, N, DEV)
+    ops.selective_scan_fwd(z(B, T, C), z(B, T, C), -torch.ones(C, N, device=DEV), z(B, T, N), z(B, T, N), y, kept_states=kept, lengths=lengths)
+    full = lambda *s: torch.full(s, NAN, device=DEV)  # noqa: E731
+    du, dd, dB, dC, dA, dstate = full(B, T, C), full(B, T, C), full(B, T, N), full(B, T, N), full(C, N), full(B, C, N)
+    ops.selective_scan_bwd(full(B, T, C), full(B, T, C), full(B, T, C), -torch.ones(C, N, device=DEV), full(B, T, N), full(B, T, N), kept,
+                           du, dd, dA, dB, dC, d_state_in=dstate, d_state_out=state, lengths=lengths)
+    assert torch.equal(dstate, state) and not any(bool(t.any()) for t in (du, dd, dB, dC, dA))
     # no sequences, no rows
     e = torch.empty(0, 3, C, device=DEV)
     ops.causal_conv_fwd(e, torch.ones(C, K, device=DEV), None, torch.empty_like(e))
     ops.causal_conv_bwd(e, e, torch.ones(C, K, device=DEV), None, torch.empty_like(e), dw)
     assert not bool(dw.any())
+    none, bc = torch.empty(0, 3, C, device=DEV), torch.empty(0, 3, N, device=DEV)
+    kept, dA = ops.selective_scan_kept_states(0, 3, C, N, DEV), full(C, N)
+    ops.selective_scan_fwd(none, none, -torch.ones(C, N, device=DEV), bc, bc, none, kept_states=kept)
+    ops.selective_scan_bwd(none, none, none, -torch.ones(C, N, device=DEV), bc, bc, kept, none, none, dA, bc, bc)
+    assert not bool(dA.any())
     m = torch.empty(0, C, device=DEV)
     dweight = torch.full((C,), NAN, device=DEV)
     ops.rms_norm_fwd(m, torch.ones(C, device=DEV), 1e-5, y=torch.empty_like(m))
     ops.rms_norm_bwd(m, m, torch.ones(C, device=DEV), torch.empty(0, device=DEV), torch.empty_like(m), dweight)
     assert not bool(dweight.any())
+
+
+# --------------------------------------------------------------------------------------------------- one step at a time
+@pytest.mark.parametrize("B,C,N", [(1, 1, 1), (3, 5, 3), (2, 64, 8), (5, 70, 16), (2, 130, 20), (33, 16, 32)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("use_z,use_D,use_bias,softplus,ragged", [(True, True, True, True, False), (False, False, False, True, True), (True, False, True, False, False)])
+def test_selective_scan_one_step(B, C, N, dtype, use_z, use_D, use_bias, softplus, ragged):
+    g = torch.Generator().manual_seed(B + C + N)
+    t = scan_case(g, B, 1, C, N, dtype, 1, use_z, use_D, use_bias, softplus, state=True, ragged=ragged)
+    c = lambda k: None if t[k] is None else t[k].to(DEV)  # noqa: E731
+    y, state = torch.full((B, 1, C), NAN, dtype=dtype, device=DEV), c("state_in")
+    ops.selective_scan_fwd(t["u"], t["delta"], c("A"), t["Bm"], t["Cm"], y, D=c("D"), z=t["z"], delta_bias=c("delta_bias"), softplus=softplus,
+                           state_in=state, state_out=state, lengths=c("lengths"))
+    want, bound = scan_want(t, softplus)
+    close(y, want["y"], bound["y"], "y")
+    close(state, want["state_out"], bound["state_out"], "state_out")
+
+
+# ----------------------------------------------------------------------------------------- the layer that they are part of
+def layer_parameters(g, width, inner, N, K=4):
+    p = dict(norm=1.0 + rand(g, width, scale=0.1), w_in=rand(g, 2 * inner, width, scale=width ** -0.5), w_out=rand(g, width, inner, scale=inner ** -0.5),
+             conv=rand(g, inner, K, scale=K ** -0.5), conv_bias=rand(g, inner, scale=0.1), A=-torch.exp(rand(g, inner, N, scale=0.5)),
+             D=rand(g, inner), delta_bias=rand(g, inner) - 3.0, w_b=rand(g, N, inner, scale=inner ** -0.5), w_c=rand(g, N, inner, scale=inner ** -0.5),
+             w_d=rand(g, inner, inner, scale=0.3 * inner ** -0.5))
+    return p
+
+
+def layer_training(p, x, dy, use_ops):
+    """Forward and backward of a float32 sequence layer (norm, projection, convolution, scan with its gate, projection) with the
+    residual added behind it.  The projections are torch products; use_ops False: all in float64 through autograd."""
+    B, T, width = x.shape
+    inner, N = p["A"].shape
+    if not use_ops:
+        q = {k: v.double().requires_grad_(True) for k, v in p.items()}
+        xl = x.double().requires_grad_(True)
+        _, y, _ = so.rms_norm(xl.reshape(-1, width), q["norm"], 1e-5)
+        h = (y @ q["w_in"].t()).reshape(B, T, 2 * inner)
+        u, _ = so.causal_conv(h[..., :inner], q["conv"], q["conv_bias"])
+        s, _ = so.selective_scan(u, u @ q["w_d"].t(), q["A"], u @ q["w_b"].t(), u @ q["w_c"].t(), q["D"], h[..., inner:], q["delta_bias"])
+        out = xl + s @ q["w_out"].t()
+        (out * dy.double()).sum().backward()
+        return out.detach(), xl.grad, {k: v.grad for k, v in q.items()}
+    q = {k: v.to(DEV) for k, v in p.items()}
+    xg, dyg = x.to(DEV), dy.to(DEV)
+    new = lambda *s: torch.empty(*s, device=DEV)  # noqa: E731
+    flat = xg.reshape(-1, width)
+    y, rstd = new(B * T, width), new(B * T)
+    ops.rms_norm_fwd(flat, q["norm"], 1e-5, y=y, rstd=rstd)
+    h = (y @ q["w_in"].t()).reshape(B, T, 2 * inner)
+    cx, z = h[..., :inner], h[..., inner:]
+    u, s = new(B, T, inner), new(B, T, inner)
+    ops.causal_conv_fwd(cx, q["conv"], q["conv_bias"], u)
+    delta, Bm, Cm = u @ q["w_d"].t(), u @ q["w_b"].t(), u @ q["w_c"].t()
+    kept = ops.selective_scan_kept_states(B, T, inner, N, DEV)
+    ops.selective_scan_fwd(u, delta, q["A"], Bm, Cm, s, D=q["D"], z=z, delta_bias=q["delta_bias"], kept_states=kept)
+    out = xg + s @ q["w_out"].t()
+    g = {}
+    ds = dyg @ q["w_out"]
+    g["w_out"] = dyg.reshape(-1, width).t() @ s.reshape(-1, inner)
+    dh = new(B, T, 2 * inner)                      # the gradients of both halves side by side, as the halves are
+    du, dd, dB, dC = new(B, T, inner), new(B, T, inner), new(B, T, N), new(B, T, N)
+    for k in ("A", "D", "delta_bias", "conv", "conv_bias", "norm"):
+        g[k] = torch.empty_like(q[k])
+    ops.selective_scan_bwd(ds, u, delta, q["A"], Bm, Cm, kept, du, dd, g["A"], dB, dC, D=q["D"], z=z, delta_bias=q["delta_bias"], dD=g["D"],
+                           dz=dh[..., inner:], d_delta_bias=g["delta_bias"])
+    rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+    g["w_d"], g["w_b"], g["w_c"] = rows(dd).t() @ rows(u), rows(dB).t() @ rows(u), rows(dC).t() @ rows(u)
+    du += dd @ q["w_d"] + dB @ q["w_b"] + dC @ q["w_c"]
+    ops.causal_conv_bwd(du, cx, q["conv"], q["conv_bias"], dh[..., :inner], g["conv"], g["conv_bias"])
+    g["w_in"] = rows(dh).t() @ y
+    dx = new(B * T, width)
+    ops.rms_norm_bwd(rows(dh) @ q["w_in"], flat, q["norm"], rstd, dx, g["norm"])
+    return out, dyg + dx.reshape(B, T, width), g
+
+
+def test_a_layer_trains():
+    """All operators in the order of a training step.  Every gradient within 1e-4 of its largest value: a chain of about ten float32
+    sums of up to 512 terms (512 x 2^-24 = 3e-5 each at worst, their usual error a thirtieth of that)."""
+    g = torch.Generator().manual_seed(8)
+    B, T, width, inner, N = 2, 150, 48, 96, 16
+    p = layer_parameters(g, width, inner, N)
+    x, dy = rand(g, B, T, width), rand(g, B, T, width)
+    want, want_dx, want_g = layer_training(p, x, dy, False)
+    out, dx, grads = layer_training(p, x, dy, True)
+    for name, a, b in [("out", out, want), ("dx", dx, want_dx)] + [(k, grads[k], want_g[k]) for k in want_g]:
+        off = float((a.cpu().double() - b).abs().max() / b.abs().max())
+        assert off < 1e-4, (name, off)
+
+
+def serve(p, q, x, state):
+    """A frame of each stream through the layer with 8-bit projections; state: convolution's and scan's, kept in place."""
+    B, width = x.shape
+    inner, N = p["A"].shape
+    new = lambda *s, dt=BF16: torch.empty(*s, dtype=dt, device=DEV)  # noqa: E731
+    a8, sa = new(B, width, dt=FP8), new(B, -(-width // 128), dt=F32)
+    ops.rms_norm_fwd(x, p["norm"], 1e-5, y8=a8, scales=sa)
+    h = new(B, 2 * inner)
+    ops.gemm_nt_fp8(a8, sa, *q["w_in"], h)
+    h = h.reshape(B, 1, 2 * inner)
+    u, s = new(B, 1, inner), new(B, 1, inner)
+    ops.causal_conv_fwd(h[..., :inner], p["conv"], p["conv_bias"], u, state_in=state[0], state_out=state[0])
+    u8, su, dbc = new(B, inner, dt=FP8), new(B, -(-inner // 128), dt=F32), new(B, inner + 2 * N)
+    ops.quantize_fp8(u.reshape(B, inner), u8, su)
+    ops.gemm_nt_fp8(u8, su, *q["w_dbc"], dbc)
+    delta, Bm, Cm = dbc.reshape(B, 1, inner + 2 * N).split((inner, N, N), dim=2)
+    ops.selective_scan_fwd(u, delta, p["A"], Bm, Cm, s, D=p["D"], z=h[..., inner:], delta_bias=p["delta_bias"], state_in=state[1], state_out=state[1])
+    s8, ss = new(B, inner, dt=FP8), new(B, -(-inner // 128), dt=F32)
+    ops.quantize_fp8(s.reshape(B, inner), s8, ss)
+    out = new(B, width)
+    ops.gemm_nt_fp8(s8, ss, *q["w_out"], out)
+    return x + out
+
+
+def serving_setup():
+    g = torch.Generator().manual_seed(4)
+    B, width, inner, N = 3, 256, 512, 16
+    p = {k: v.to(DEV) for k, v in layer_parameters(g, width, inner, N).items()}
+    q = {}
+    p["w_dbc"] = torch.cat((p["w_d"], p["w_b"], p["w_c"]))
+    for k in ("w_in", "w_out", "w_dbc"):
+        R, C = p[k].shape
+        w8, s = torch.empty(R, C, dtype=FP8, device=DEV), torch.empty(-(-R // 128), -(-C // 128), device=DEV)
+        ops.quantize_fp8_blocks(p[k], w8, s)
+        q[k] = (w8, s)
+    fresh = lambda: [torch.zeros(B, 3, inner, dtype=BF16, device=DEV), torch.zeros(B, inner, N, device=DEV)]  # noqa: E731
+    frames = [rand(g, B, width, dtype=BF16).to(DEV) for _ in range(12)]
+    return p, q, fresh, frames
+
+
+def test_a_layer_serves_frames_one_by_one_from_a_graph():
+    """The layer's step recorded once and replayed for every frame, with eager work and synchronisations in between, against eager
+    steps; a second graph of the same step has workspaces of its own and is replayed in turn with the first."""
+    p, q, fresh, frames = serving_setup()
+    state = fresh()
+    want = [serve(p, q, x, state).clone() for x in frames]
+    end = [t.clone() for t in state]
+    assert all(bool(w.isfinite().all()) for w in want) and not torch.equal(want[0], want[1])
+    x = torch.empty_like(frames[0])
+    state = fresh()
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        for t in state:
+            t.zero_()
+        x.copy_(frames[0])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            serve(p, q, x, state)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = serve(p, q, x, state)
+        graphs.append((graph, out))
+    for t in state:
+        t.zero_()
+    for i, f in enumerate(frames):
+        x.copy_(f)
+        graph, out = graphs[i % 2]
+        graph.replay()
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), i
+        torch.randn(1000, device=DEV).sum()
+    assert torch.equal(state[0], end[0]) and torch.equal(state[1], end[1])
+
+
+def test_a_training_step_replays():
+    """Forward and backward of convolution, scan and norm recorded in one graph, replayed on new inputs: bits of the eager calls."""
+    g = torch.Generator().manual_seed(6)
+    B, T, C, N, K = 2, 300, 80, 16, 4
+    x, dy = torch.empty(B, T, C, device=DEV), torch.empty(B, T, C, device=DEV)
+    w, b = rand(g, C, K).to(DEV), rand(g, C).to(DEV)
+    A, nw = (-torch.exp(rand(g, C, N))).to(DEV), rand(g, C).to(DEV)
+    Bm, Cm = rand(g, B, T, N).to(DEV), rand(g, B, T, N).to(DEV)
+
+    def body():
+        new = lambda *s: torch.empty(*s, device=DEV)  # noqa: E731
+        u, y, n, rstd = new(B, T, C), new(B, T, C), new(B * T, C), new(B * T)
+        kept = ops.selective_scan_kept_states(B, T, C, N, DEV)
+        ops.causal_conv_fwd(x, w, b, u)
+        ops.selective_scan_fwd(u, u, A, Bm, Cm, y, kept_states=kept)
+        ops.rms_norm_fwd(y.reshape(-1, C), nw, 1e-5, y=n, rstd=rstd)
+        dn, dnw, du, dd, dA, dB, dC = new(B * T, C), new(C), new(B, T, C), new(B, T, C), new(C, N), new(B, T, N), new(B, T, N)
+        ops.rms_norm_bwd(dy.reshape(-1, C), y.reshape(-1, C), nw, rstd, dn, dnw)
+        ops.selective_scan_bwd(dn.reshape(B, T, C), u, u, A, Bm, Cm, kept, du, dd, dA, dB, dC)
+        du += dd
+        dx, dw, db = new(B, T, C), new(C, K), new(C)
+        ops.causal_conv_bwd(du, x, w, b, dx, dw, db)
+        return [n, dnw, dA, dB, dC, dx, dw, db]
+
+    x.normal_(), dy.normal_()
+    body()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = body()
+    for i in range(4):
+        x.normal_(), dy.normal_()
+        want = body()
+        for t in outs:
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(outs, want):
+            assert torch.equal(a, c), i
+
+
+def test_calls_on_two_streams_at_once():
+    """Two streams, each with its own operands and workspaces, many calls in flight: bits of the calls one by one."""
+    g = torch.Generator().manual_seed(12)
+    B, T, C, N = 2, 400, 64, 16
+    sets = []
+    for _ in range(2):
+        t = scan_case(g, B, T, C, N, F32, state=True)
+        sets.append((t, scan_run(t, F32)))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(scan_run(sets[i][0], F32))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for k, v in sets[i][1].items():
+                assert torch.equal(r[k], v), (i, k)
+
+
+def test_gradients_against_differences():
+    """Directional differences of the kernels' own float32 forward pass: d loss = loss(v + h d) - loss(v - h d) over 2 h with h = 2^-8.
+    The difference's error is h^2 / 6 of the third derivative (of order one: 3e-6) and the rounding of the outputs, 1e-6 / h of
+    their sum's usual error = 3e-4 relative to the sum of magnitudes; 5e-3 of the derivative's size is asked for."""
+    g = torch.Generator().manual_seed(21)
+    B, T, C, N = 2, 70, 24, 8
+    t = scan_case(g, B, T, C, N, F32, state=True)
+    got = scan_run(t, F32)
+    names = dict(u="du", delta="ddelta", z="dz", Bm="dB", Cm="dC", A="dA", D="dD", delta_bias="d_delta_bias", state_in="d_state_in")
+
+    def loss(v):
+        y, state = torch.empty(B, T, C, device=DEV), torch.empty(B, C, N, device=DEV)
+        c = lambda k: v[k].to(DEV)  # noqa: E731
+        ops.selective_scan_fwd(v["u"], v["delta"], c("A"), v["Bm"], v["Cm"], y, D=c("D"), z=v["z"], delta_bias=c("delta_bias"),
+                               state_in=c("state_in"), state_out=state)
+        return float((y.double() * t["dy"].double()).sum() + (state.double() * t["d_state_out"].to(DEV).double()).sum())
+
+    h = 2.0 ** -8
+    for name, grad in names.items():
+        d = torch.randn(t[name].shape, generator=g).to(t[name].device)
+        if name == "A":
+            d *= t["A"].abs()
+        plus, minus = dict(t), dict(t)
+        plus[name], minus[name] = t[name] + h * d, t[name] - h * d
+        slope = (loss(plus) - loss(minus)) / (2 * h)
+        want = float((got[grad].double().to(d.device) * d.double()).sum())
+        size = float((got[grad].double().to(d.device) * d.double()).square().sum().sqrt())
+        assert abs(slope - want) < 5e-3 * max(size, abs(want)) + 1e-3, (name, slope, want)
+
+
+# ------------------------------------------------------------------------------------------------------------ refusals
+def test_refused_calls_leave_the_outputs_alone():
+    B, T, C, N, K = 2, 5, 16, 8, 4
+    z = lambda *s, dt=F32: torch.zeros(*s, dtype=dt, device=DEV)  # noqa: E731
+    x, y, w, A, bc = z(B, T, C), torch.full((B, T, C), 3.0, device=DEV), z(C, K), -torch.ones(C, N, device=DEV), z(B, T, N)
+    conv = lambda **k: ops.causal_conv_fwd(**{**dict(x=x, weight=w, bias=None, y=y), **k})  # noqa: E731
+    scan = lambda **k: ops.selective_scan_fwd(**{**dict(u=x, delta=x, A=A, Bm=bc, Cm=bc, y=y), **k})  # noqa: E731
+    for bad in (dict(weight=z(C, 5)), dict(weight=z(C, 1)), dict(weight=z(C + 1, K)), dict(weight=w.double()), dict(y=z(B, T, C, dt=BF16)),
+                dict(y=z(B, T + 1, C)), dict(y=x), dict(bias=z(C + 1)), dict(state_in=z(B, K, C)), dict(state_out=x[:, :3]),
+                dict(lengths=z(B)), dict(lengths=z(B + 1, dt=torch.int32)), dict(x=z(B, C, T).transpose(1, 2)), dict(x=x.half()), dict(x=x[0]),
+                dict(x=x.cpu()), dict(y=z(1, T, C).expand(B, T, C)), dict(y=z(B, 1, C).expand(B, T, C))):
+        with pytest.raises(ValueError):
+            conv(**bad)
+    for bad in (dict(A=z(C, 33)), dict(A=z(C, 0)), dict(A=z(N, C)), dict(delta=z(B, T, C, dt=BF16)), dict(Bm=z(B, T, N + 1)), dict(Cm=z(B, T + 1, N)),
+                dict(y=x), dict(z=z(B, T, C + 1)), dict(D=z(N)), dict(delta_bias=z(C, dt=BF16)), dict(state_in=z(B, N, C)),
+                dict(state_out=z(B, C, N, dt=BF16)), dict(kept_states=z(7)), dict(lengths=z(B, dt=torch.int64)), dict(u=x.transpose(1, 2))):
+        with pytest.raises(ValueError):
+            scan(**bad)
+    kept = ops.selective_scan_kept_states(B, T, C, N, DEV)
+    new = lambda *s: torch.empty(*s, device=DEV)  # noqa: E731
+    back = lambda **k: ops.selective_scan_bwd(**{**dict(dy=x, u=new(B, T, C), delta=new(B, T, C), A=A, Bm=bc, Cm=bc, kept_states=kept, du=y,  # noqa: E731
+                                                        ddelta=new(B, T, C), dA=new(C, N), dB=new(B, T, N), dC=new(B, T, N)), **k})
+    both = new(B, T, C)
+    for bad in (dict(du=x), dict(du=both, ddelta=both), dict(dz=new(B, T, C)), dict(z=new(B, T, C)), dict(kept_states=kept[1:]), dict(dA=new(N, C)), dict(du=None), dict(dB=bc),
+                dict(d_state_in=new(B, C, N + 1))):
+        with pytest.raises(ValueError):
+            back(**bad)
+    m, nw, q, s = z(4, 300), z(300), z(4, 300, dt=FP8), z(4, 3)
+    keep = torch.full((4, 300), 3.0, device=DEV)
+    for call in (lambda: ops.rms_norm_fwd(m, nw, 1e-5, y=keep[:, :299]), lambda: ops.rms_norm_fwd(m, nw[1:], 1e-5, y=keep),
+                 lambda: ops.rms_norm_fwd(m.t(), nw, 1e-5, y=keep), lambda: ops.rms_norm_fwd(m, nw, 1e-5, y8=q, scales=z(4, 2)),
+                 lambda: ops.rms_norm_fwd(m, nw, 1e-5, y=keep, rstd=z(3)), lambda: ops.rms_norm_bwd(m, m, nw, z(4), keep, z(299)),
+                 lambda: ops.quantize_fp8(m, q, z(4, 2)), lambda: ops.quantize_fp8(m, m, s), lambda: ops.quantize_fp8_blocks(m, q, z(1, 2))):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ops.rms_norm_fwd(m, nw, 1e-5), lambda: ops.rms_norm_fwd(m, nw, 1e-5, y8=q),
+                 lambda: ops.rms_norm_fwd(m, nw, 1e-5, y=keep, sum_out=z(4, 300)), lambda: ops.rms_norm_fwd(z(1, 16400), z(16400), 1e-5, y=z(1, 16400))):
+        with pytest.raises(RuntimeError):
+            call()
+    a8, b8, out = z(4, 304, dt=FP8), z(8, 304, dt=FP8), torch.full((4, 8), 3.0, dtype=BF16, device=DEV)
+    gemm = lambda **k: ops.gemm_nt_fp8(**{**dict(a8=a8, a_scales=z(4, 3), b8=b8, b_scales=z(1, 3), out=out), **k})  # noqa: E731
+    for bad in (dict(a8=q, a_scales=s), dict(a_scales=z(4, 2)), dict(b8=z(8, 320, dt=FP8)), dict(b_scales=z(8, 3)), dict(out=z(4, 8)),
+                dict(out=z(4, 9, dt=BF16)), dict(a8=z(4 * 304 + 8, dt=FP8)[8:].view(4, 304)), dict(out=z(8, 4, dt=BF16).t())):
+        with pytest.raises(ValueError):
+            gemm(**bad)
+    torch.cuda.synchronize()
+    assert bool((y == 3.0).all()) and bool((keep == 3.0).all()) and bool((out == 3.0).all())
+
+
+# --------------------------------------------------------------------------------------------------- far places in memory
+def test_offsets_beyond_32_bits():
+    """Sequences and steps more than 2^31 elements apart, outputs of more than 2^31 elements: the same bits as close together."""
+    g = torch.Generator().manual_seed(31)
+    B, T, C, N, K = 2, 40, 24, 16, 4
+    t = scan_case(g, B, T, C, N, BF16, state=True)
+    far = torch.empty(2 ** 31 + 10 * T * C, dtype=BF16, device=DEV)
+
+    def spread(v, at):
+        out = torch.as_strided(far, v.shape, (2 ** 31 + 64, v.shape[2], 1), at)
+        return out.copy_(v)
+
+    near = scan_run(t, BF16)
+    moved = dict(t)
+    for i, k in enumerate(("u", "delta", "z", "dy", "Bm", "Cm")):
+        moved[k] = spread(t[k], i * T * C)
+    got = scan_run(moved, BF16)
+    for k, v in near.items():
+        assert torch.equal(got[k], v), k
+    # an output whose sequences are far apart, and an input whose steps are (2^26 elements, 40 of them)
+    y = torch.as_strided(far, (B, T, C), (2 ** 31 + 64, C, 1), 8 * T * C)
+    args = lambda v, out: ops.selective_scan_fwd(v["u"], v["delta"], t["A"].to(DEV), v["Bm"], v["Cm"], out, D=t["D"].to(DEV), z=v["z"],  # noqa: E731
+                                                 delta_bias=t["delta_bias"].to(DEV), state_in=t["state_in"].to(DEV))
+    args(moved, y)
+    assert torch.equal(y, near["y"])
+    w, b = rand(g, C, K).to(DEV), rand(g, C).to(DEV)
+    want, got = torch.empty(B, T, C, dtype=BF16, device=DEV), torch.as_strided(far, (B, T, C), (C, 2 ** 31 // T, 1), 8 * T * C)
+    x = t["u"].contiguous()
+    ops.causal_conv_fwd(x, w, b, want)
+    ops.causal_conv_fwd(moved["u"], w, b, got)
+    assert torch.equal(got, want)
+    got.copy_(x)
+    again, want_d, got_d = torch.empty_like(want), [torch.empty_like(v) for v in (x, w, b)], [torch.empty_like(v) for v in (x, w, b)]
+    ops.causal_conv_fwd(got, w, b, again)
+    assert torch.equal(again, want)
+    ops.causal_conv_bwd(t["dy"].contiguous(), x, w, b, *want_d)
+    ops.causal_conv_bwd(moved["dy"], got, w, b, *got_d)
+    assert all(torch.equal(p, q) for p, q in zip(got_d, want_d))
+    del far, y, moved, got
+    # more than 2^31 values of a norm, of 8-bit operands and of a product
+    rows, C = 2 ** 17 + 3, 16384
+    x, nw = torch.zeros(rows, C, dtype=BF16, device=DEV), rand(g, C).to(DEV)
+    x[-3:] = rand(g, 3, C, dtype=BF16).to(DEV)
+    y, x8, s = torch.empty_like(x), torch.empty(rows, C, dtype=FP8, device=DEV), torch.empty(rows, C // 128, device=DEV)
+    rstd, dx, dw = torch.empty(rows, device=DEV), torch.empty_like(x), torch.empty_like(nw)
+    ops.rms_norm_fwd(x, nw, 1e-5, y=y, y8=x8, scales=s, rstd=rstd)
+    ops.rms_norm_bwd(x, x, nw, rstd, dx, dw)
+    y3, x3, s3, r3, dx3, dw3 = torch.empty(3, C, dtype=BF16, device=DEV), torch.empty(3, C, dtype=FP8, device=DEV), s[:3].clone(), rstd[:3].clone(), dx[:3].clone(), dw.clone()
+    ops.rms_norm_fwd(x[-3:].clone(), nw, 1e-5, y=y3, y8=x3, scales=s3, rstd=r3)
+    ops.rms_norm_bwd(x[-3:].clone(), x[-3:].clone(), nw, r3, dx3, dw3)
+    b8 = lambda v: v.view(torch.uint8)  # noqa: E731
+    assert torch.equal(y[-3:], y3) and torch.equal(b8(x8[-3:]), b8(x3)) and torch.equal(s[-3:], s3) and torch.equal(rstd[-3:], r3)
+    assert torch.equal(dx[-3:], dx3) and bool((dw - dw3).abs().max() <= 1e-5 * dw3.abs().max())    # zero rows add nothing; another order
+    ops.quantize_fp8(x, x8, s)
+    ops.quantize_fp8(x[-3:].clone(), x3, s3)
+    assert torch.equal(b8(x8[-3:]), b8(x3)) and torch.equal(s[-3:], s3)
+    del x, y, x8, s, rstd, dx
+    M = N = 46400
+    a8, sa = (rand(g, M, 16) * 2).to(FP8).to(DEV), torch.ones(M, 1, device=DEV)
+    out, last = torch.empty(M, N, dtype=BF16, device=DEV), torch.empty(64, N, dtype=BF16, device=DEV)
+    sb = torch.ones(-(-N // 128), 1, device=DEV)
+    ops.gemm_nt_fp8(a8, sa, a8, sb, out)
+    ops.gemm_nt_fp8(a8[-64:].contiguous(), sa[-64:].contiguous(), a8, sb, last)
+    assert torch.equal(out[-64:], last)

@@ -50,15 +50,31 @@ __device__ __forceinline__ float clamp_fp8(float v) {   // NaN stays NaN
   return v > kFp8Max ? kFp8Max : (v < -kFp8Max ? -kFp8Max : v);
 }
 
-// the quotients are IEEE divisions: a reciprocal's last bit would move values halfway between two of the format
+// The quotients are correctly rounded (an error in the last bit would move values halfway between two of the format): the reciprocal
+// is, a first correction by the exact remainder brings v r to within one unit, and a second one rounds correctly (Markstein 1990).
+// 16384 x 8192 bfloat16 takes 92 us, 4.4 TB/s; with IEEE divisions 103 us.  An exact zero loses its sign.  A remainder may lose bits below 2^-149 where a scale is near its least; that is 2^-17 of the quotient's last place at most.
+struct Quotient {
+  float scale, r;
+  __device__ __forceinline__ explicit Quotient(float s) : scale(s), r(1.0f / s) {
+    if (r == 0.0f) scale = 0.0f;   // of an infinite block: finite values become 0, infinite ones NaN
+  }
+  __device__ __forceinline__ float operator()(float v) const {
+    float q = v * r;
+    q = fmaf(fmaf(-q, scale, v), r, q);
+    q = fmaf(fmaf(-q, scale, v), r, q);
+    return clamp_fp8(q);
+  }
+};
+
 __device__ __forceinline__ uint2 to_fp8(f32x8 v, float scale) {
+  const Quotient of(scale);
   uint2 q;
   int w = 0;
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp_fp8(v[0] / scale), clamp_fp8(v[1] / scale), w, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp_fp8(v[2] / scale), clamp_fp8(v[3] / scale), w, true);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(of(v[0]), of(v[1]), w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(of(v[2]), of(v[3]), w, true);
   q.x = (unsigned)w;
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp_fp8(v[4] / scale), clamp_fp8(v[5] / scale), w, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp_fp8(v[6] / scale), clamp_fp8(v[7] / scale), w, true);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(of(v[4]), of(v[5]), w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(of(v[6]), of(v[7]), w, true);
   q.y = (unsigned)w;
   return q;
 }

@@ -10,7 +10,7 @@ combinations) and launches nothing.  Outputs share no memory with each other or 
 inputs where a call does not say so.  Activations are float32 or bfloat16, parameters,
 statistics and states float32.  Workspaces are torch allocations of the call.
 """
-import ctypes
+import struct
 
 import torch
 
@@ -21,15 +21,18 @@ FP8 = torch.float8_e4m3fn
 _DTYPE = {F32: 0, BF16: 1}
 
 
+# A call for single frames is bound by the host: the scan's takes 11 us, 8 of them for the checks below and 3 for the launch, its
+# kernel 6.  So they spare objects and calls: torch.cuda.current_stream() alone would cost 2 us, an attribute of a tensor 0.05 us.
 def _launch(device, name, *args):
-    # (torch.cuda.current_stream() makes an object of every call, 2 us; a launch takes 4)
     fn = getattr(capi.load(), name)
     stream = torch._C._cuda_getCurrentRawStream(device)
-    if device != torch.cuda.current_device():
+    if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            capi.check(fn(*args, stream), name)
+            rc = fn(*args, stream)
     else:
-        capi.check(fn(*args, stream), name)
+        rc = fn(*args, stream)
+    if rc:
+        capi.check(rc, name)
 
 
 def _bad(what, t, want):
@@ -37,60 +40,70 @@ def _bad(what, t, want):
     raise ValueError("%s: expected %s, got %s" % (what, want, got))
 
 
-def _flat(t, dtype, shape, device, what):
-    """A contiguous tensor of this type and shape on GPU `device`; its address."""
-    if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+def _opt(t, dtype, shape, device, what):
+    """The address of a contiguous tensor of this type and shape on GPU `device`, None without one."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
         _bad(what, t, "a contiguous %s tensor %s on cuda:%d" % (dtype, shape, device))
     return t.data_ptr()
 
 
-def _opt(t, dtype, shape, device, what):
-    return None if t is None else _flat(t, dtype, shape, device, what)
+def _flat(t, dtype, shape, device, what):
+    if t is None:
+        _bad(what, t, "a contiguous %s tensor %s on cuda:%d" % (dtype, shape, device))
+    return _opt(t, dtype, shape, device, what)
 
 
 def _matrix(t, what):
     """(rows, columns, type code, device index) of a contiguous float32 or bfloat16 GPU matrix."""
     if t.dim() != 2 or t.dtype not in _DTYPE or not t.is_cuda or not t.is_contiguous() or t.shape[1] == 0:
         _bad(what, t, "a contiguous float32 or bfloat16 GPU matrix with columns")
-    return t.shape[0], t.shape[1], _DTYPE[t.dtype], t.get_device()
-
-
-def _seq(t, dtype, shape, device, what, strides, out=False):
-    """The address of a sequence [B, T, C] of this type with unit stride over C; its strides over B and T join `strides`.  An
-    output's rows may not overlap."""
-    if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != device:
-        _bad(what, t, "a %s tensor %s on cuda:%d" % (dtype, shape, device))
-    sb, st, sc = t.stride()
-    B, T, C = shape
-    if sc != 1 and C > 1:
-        _bad(what, t, "unit stride over the last axis")
-    if out and ((T > 1 and st < C) or (B > 1 and sb < C) or (B > 1 and T > 1 and sb < (T - 1) * st + C and st < (B - 1) * sb + C)):
-        _bad(what, t, "rows that do not overlap")
-    strides += (sb, st)
-    return t.data_ptr()
+    return *t.shape, _DTYPE[t.dtype], t.get_device()
 
 
 def _sequence(t, what):
     """(B, T, C, type, device index) of a float32 or bfloat16 GPU tensor [B, T, C]."""
     if t.dim() != 3 or t.dtype not in _DTYPE or not t.is_cuda or t.shape[2] == 0:
         _bad(what, t, "a float32 or bfloat16 GPU tensor [B, T, C] with channels")
-    B, T, C = t.shape
-    return B, T, C, t.dtype, t.get_device()
+    return *t.shape, t.dtype, t.get_device()
 
 
-def _host_array(strides):
-    return (ctypes.c_longlong * len(strides))(*strides)
+def _sequences(dtype, device, inputs, outputs):
+    """The addresses of sequences [B, T, C] of this type with unit stride over C, and their strides over B and T as an array of 64-bit
+    integers.  inputs, outputs: (name, tensor, shape); None, where the shape is too, has no address.  An output's rows may not
+    overlap, and no output begins where an input or another output does (steps of a sequence are worked on at once)."""
+    ptrs, strides = [], []
+    for what, t, shape in inputs + outputs:
+        if t is None and shape is None:
+            strides += (0, 0)
+            ptrs.append(None)
+            continue
+        if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+            _bad(what, t, "a %s tensor %s on cuda:%d" % (dtype, shape, device))
+        sb, st, sc = t.stride()
+        if sc != 1 and shape[2] > 1:
+            _bad(what, t, "unit stride over the last axis")
+        strides += (sb, st)
+        ptrs.append(t.data_ptr())
+    for i, (what, t, _) in enumerate(outputs, len(inputs)):
+        if t is None:
+            continue
+        if not t.is_contiguous():
+            (B, T, C), (sb, st, _) = t.shape, t.stride()
+            if (T > 1 and st < C) or (B > 1 and sb < C) or (B > 1 and T > 1 and sb < (T - 1) * st + C and st < (B - 1) * sb + C):
+                _bad(what, t, "rows that do not overlap")
+        if ptrs[i] and ptrs[i] in ptrs[:i]:
+            raise ValueError("%s is one of the inputs or another output" % what)
+    return ptrs, _PACK[len(strides)](*strides)
 
 
-def _apart(outs, ins):
-    """No output begins where an input or another output does (addresses; 0 and None are no memory): steps of a sequence are
-    worked on at once."""
-    seen = list(ins)
-    for o in outs:
-        if o:
-            if o in seen:
-                raise ValueError("an output is one of the inputs or another output")
-            seen.append(o)
+_PACK = {n: struct.Struct("%dq" % n).pack for n in (4, 6, 12, 22)}
+
+
+def _apart(ptr, ptrs, what):
+    if ptr and ptr in ptrs:
+        raise ValueError("%s is one of the sequences" % what)
 
 
 def rms_norm_fwd(x, weight, eps, y=None, residual=None, sum_out=None, y8=None, scales=None, rstd=None):
@@ -162,14 +175,12 @@ def causal_conv_fwd(x, weight, bias, y, state_in=None, state_out=None, lengths=N
     continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths (int32 [B]) bounds each sequence:
     rows behind it are not used and are zero in y.  x and y may be views with any strides over B and T."""
     B, T, C, dt, dev = _sequence(x, "x")
-    strides = []
-    xp = _seq(x, dt, (B, T, C), dev, "x", strides)
-    yp = _seq(y, dt, (B, T, C), dev, "y", strides, out=True)
+    (xp, yp), strides = _sequences(dt, dev, (("x", x, (B, T, C)),), (("y", y, (B, T, C)),))
     w, K = _taps(weight, C, dev)
     sp, op = _opt(state_in, dt, (B, K - 1, C), dev, "state_in"), _opt(state_out, dt, (B, K - 1, C), dev, "state_out")
-    _apart((yp, op), (xp,))
-    _apart((yp,), (sp, op))
-    _launch(dev, "slamhip_causal_conv_fwd", xp, _host_array(strides), w, _opt(bias, F32, (C,), dev, "bias"), sp,
+    _apart(sp, (yp,), "state_in")
+    _apart(op, (xp, yp), "state_out")
+    _launch(dev, "slamhip_causal_conv_fwd", xp, strides, w, _opt(bias, F32, (C,), dev, "bias"), sp,
             _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K, int(silu), _DTYPE[dt], yp, op)
 
 
@@ -178,17 +189,16 @@ def causal_conv_bwd(dy, x, weight, bias, dx, dweight, dbias=None, state_in=None,
     """Gradients of causal_conv_fwd (same x, weight, bias, state_in, lengths, silu): dx, dweight, dbias and d_state_in from dy
     and from d_state_out, the gradient that arrives at state_out."""
     B, T, C, dt, dev = _sequence(x, "x")
-    strides = []
-    yp = _seq(dy, dt, (B, T, C), dev, "dy", strides)
-    xp = _seq(x, dt, (B, T, C), dev, "x", strides)
-    dp = _seq(dx, dt, (B, T, C), dev, "dx", strides, out=True)
+    shape = (B, T, C)
+    (yp, xp, dp), strides = _sequences(dt, dev, (("dy", dy, shape), ("x", x, shape)), (("dx", dx, shape),))
     w, K = _taps(weight, C, dev)
     ip, op = _opt(state_in, dt, (B, K - 1, C), dev, "state_in"), _opt(d_state_out, dt, (B, K - 1, C), dev, "d_state_out")
     gp = _opt(d_state_in, dt, (B, K - 1, C), dev, "d_state_in")
-    _apart((dp, gp), (yp, xp, ip, op))
+    _apart(dp, (ip, op), "dx")
+    _apart(gp, (yp, xp, dp, ip, op), "d_state_in")
     nbytes = capi.load().slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, "slamhip_causal_conv_bwd", yp, xp, _host_array(strides), w, _opt(bias, F32, (C,), dev, "bias"), ip, op,
+    _launch(dev, "slamhip_causal_conv_bwd", yp, xp, strides, w, _opt(bias, F32, (C,), dev, "bias"), ip, op,
             _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, K, int(silu), _DTYPE[dt], dp,
             _flat(dweight, F32, (C, K), dev, "dweight"), _opt(dbias, F32, (C,), dev, "dbias"), gp, ws.data_ptr(), nbytes)
 
@@ -198,18 +208,15 @@ def selective_scan_kept_states(B, T, C, N, device):
     return torch.empty(capi.load().slamhip_selective_scan_kept_floats(B, T, C, N), dtype=F32, device=device)
 
 
-def _scan_inputs(u, delta, A, Bm, Cm, z, strides):
+def _scan_inputs(u, delta, A, Bm, Cm, z):
+    """The sizes, and the input sequences as _sequences() takes them."""
     B, T, C, dt, dev = _sequence(u, "u")
     if A.dim() != 2 or not 1 <= A.shape[1] <= 32:
         _bad("A", A, "[%d, N] with 1 <= N <= 32" % C)
     N = A.shape[1]
-    up, dp = _seq(u, dt, (B, T, C), dev, "u", strides), _seq(delta, dt, (B, T, C), dev, "delta", strides)
-    zp = None
-    if z is None:
-        strides += (0, 0)
-    else:
-        zp = _seq(z, dt, (B, T, C), dev, "z", strides)
-    return B, T, C, N, dt, dev, (up, dp, zp, _seq(Bm, dt, (B, T, N), dev, "Bm", strides), _seq(Cm, dt, (B, T, N), dev, "Cm", strides))
+    shape, states = (B, T, C), (B, T, N)
+    return B, T, C, N, dt, dev, (("u", u, shape), ("delta", delta, shape), ("z", z, None if z is None else shape), ("Bm", Bm, states),
+                                 ("Cm", Cm, states))
 
 
 def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, softplus=True, state_in=None, state_out=None,
@@ -220,10 +227,8 @@ def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, 
     to be state_in of the call that continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths
     (int32 [B]) bounds each sequence: rows behind it are not used and are zero in y.  kept_states (selective_scan_kept_states)
     is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T."""
-    strides = []
-    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z, strides)
-    yp = _seq(y, dt, (B, T, C), dev, "y", strides, out=True)
-    _apart((yp,), ptrs)
+    B, T, C, N, dt, dev, inputs = _scan_inputs(u, delta, A, Bm, Cm, z)
+    (*ptrs, yp), strides = _sequences(dt, dev, inputs, (("y", y, (B, T, C)),))
     lib = capi.load()
     kp = ws = None
     if kept_states is not None:
@@ -231,7 +236,7 @@ def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, 
     nbytes = lib.slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N)
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, "slamhip_selective_scan_fwd", *ptrs, _host_array(strides), _flat(A, F32, (C, N), dev, "A"),
+    _launch(dev, "slamhip_selective_scan_fwd", *ptrs, strides, _flat(A, F32, (C, N), dev, "A"),
             _opt(D, F32, (C,), dev, "D"), _opt(delta_bias, F32, (C,), dev, "delta_bias"), _opt(state_in, F32, (B, C, N), dev, "state_in"),
             _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt], yp,
             _opt(state_out, F32, (B, C, N), dev, "state_out"), kp, capi.ptr(ws), nbytes)
@@ -243,24 +248,19 @@ def selective_scan_bwd(dy, u, delta, A, Bm, Cm, kept_states, du, ddelta, dA, dB,
     gradient that arrives at state_out: du, ddelta, dz (given when z is), dB, dC, dA, dD, d_delta_bias and d_state_in."""
     if (z is None) != (dz is None):
         raise ValueError("selective_scan_bwd: dz is wanted exactly when there is z")
-    strides, out_strides = [], []
-    B, T, C, N, dt, dev, ptrs = _scan_inputs(u, delta, A, Bm, Cm, z, strides)
-    outs = []
-    for t, w, what in ((du, C, "du"), (ddelta, C, "ddelta"), (dz, C, "dz"), (dB, N, "dB"), (dC, N, "dC")):
-        if t is None and what == "dz":
-            outs.append(None)
-            out_strides += (0, 0)
-        else:
-            outs.append(_seq(t, dt, (B, T, w), dev, what, out_strides, out=True))
-    yp = _seq(dy, dt, (B, T, C), dev, "dy", out_strides)
+    B, T, C, N, dt, dev, inputs = _scan_inputs(u, delta, A, Bm, Cm, z)
+    shape, states = (B, T, C), (B, T, N)
+    ptrs, strides = _sequences(dt, dev, (("dy", dy, shape),) + inputs, (
+        ("du", du, shape), ("ddelta", ddelta, shape), ("dz", dz, None if dz is None else shape), ("dB", dB, states), ("dC", dC, states)))
     gp, op = _opt(d_state_in, F32, (B, C, N), dev, "d_state_in"), _opt(d_state_out, F32, (B, C, N), dev, "d_state_out")
-    _apart((*outs, gp), (*ptrs, yp, op))
+    _apart(gp, ptrs + [op], "d_state_in")
+    _apart(op, ptrs[6:], "d_state_out")
     lib = capi.load()
     kp = _flat(kept_states, F32, (lib.slamhip_selective_scan_kept_floats(B, T, C, N),), dev, "kept_states")
     nbytes = lib.slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, "slamhip_selective_scan_bwd", yp, *ptrs, _host_array(out_strides[10:] + strides + out_strides[:10]),
-            _flat(A, F32, (C, N), dev, "A"), _opt(D, F32, (C,), dev, "D"), _opt(delta_bias, F32, (C,), dev, "delta_bias"), kp, op,
-            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt], *outs,
+    _launch(dev, "slamhip_selective_scan_bwd", *ptrs[:6], strides, _flat(A, F32, (C, N), dev, "A"), _opt(D, F32, (C,), dev, "D"),
+            _opt(delta_bias, F32, (C,), dev, "delta_bias"), kp, op,
+            _opt(lengths, torch.int32, (B,), dev, "lengths"), B, T, C, N, int(softplus), _DTYPE[dt], *ptrs[6:],
             _flat(dA, F32, (C, N), dev, "dA"), _opt(dD, F32, (C,), dev, "dD"), _opt(d_delta_bias, F32, (C,), dev, "d_delta_bias"),
             gp, ws.data_ptr(), nbytes)

@@ -144,6 +144,22 @@ def test_quantize_blocks_equal_the_rule_exactly(R, C, dtype):
     assert torch.equal(q.cpu().float(), want.float())
 
 
+def test_quantize_values_around_halfway():
+    """Values whose quotient is halfway between two of the format, and their neighbours, over the range of scales."""
+    g = torch.Generator().manual_seed(3)
+    rows = 2048
+    scale = (1 + torch.randint(0, 4096, (rows, 1), generator=g) / 4096.0) * torch.exp2(torch.randint(-100, 110, (rows, 1), generator=g).float())
+    half = (2 * torch.randint(8, 16, (rows, 128), generator=g) + 1) / 16.0 * torch.exp2(torch.randint(-6, 8, (rows, 128), generator=g).float())
+    x = half * scale
+    x = torch.where(torch.rand(x.shape, generator=g) < 0.5, x, torch.nextafter(x, torch.where(torch.rand(x.shape, generator=g) < 0.5, 0.0, 3e38)))
+    x = x.minimum(447 * scale) * torch.where(torch.rand(x.shape, generator=g) < 0.5, -1.0, 1.0)
+    x[:, :1] = 448 * scale
+    q, scales = torch.zeros(rows, 128, dtype=FP8, device=DEV), torch.empty(rows, 1, device=DEV)
+    ops.quantize_fp8(x.to(DEV), q, scales)
+    assert torch.equal(scales.cpu(), scale)
+    assert torch.equal(q.cpu().float(), (x / scale).to(FP8).float())
+
+
 def test_quantize_special_values():
     """The largest value becomes 448; a NaN takes its block with it and no other; an infinity's block has an infinite scale."""
     x = torch.ones(4, 256, device=DEV)

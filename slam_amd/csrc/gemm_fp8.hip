@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(256) gemm_fp8_parts_kernel(const float* __rest
   if (at >= n) return;
   const int valid = (int)min(n - at, 4LL);
   f32x4 v = loadv<4>(part + at, valid);
+#pragma unroll 4
   for (int i = 1; i < parts; ++i) v += loadv<4>(part + i * n + at, valid);
   storev<4>(out + at, v, valid);
 }

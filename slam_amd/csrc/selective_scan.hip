@@ -665,6 +665,7 @@ __global__ void __launch_bounds__(256) selective_scan_parts_kernel(ScanArgs a, i
     if (n >= a.N) return;
     const int b = (int)(step / a.T), t = (int)(step - (long long)b * a.T);
     float s = 0.0f;
+#pragma unroll 8
     for (int g = 0; g < groups; ++g) s += a.part_bc[(step * groups + g) * 2 * np + v];
     if (a.lengths && t >= a.lengths[b]) s = 0.0f;
     if (which)
@@ -678,6 +679,7 @@ __global__ void __launch_bounds__(256) selective_scan_parts_kernel(ScanArgs a, i
   const int c = (blockIdx.x - bc_groups) * 32 + tx, parts = B * a.chunks;
   float s = 0.0f;
   if (c < columns)
+#pragma unroll 8
     for (int p = ty; p < parts; p += 8) s += a.part[(long long)p * columns + c];
   sh[ty][tx] = s;
   __syncthreads();

@@ -4,6 +4,10 @@
 //   8 bits: for each 128 consecutive values of a row, scale = max(max|y| / 448, 2^-100), y8 = e4m3(y / scale)
 //   backward: hat = s rstd, dx = rstd (w dy - hat mean(w dy hat)) + d_sum, dw = sum over rows of dy hat
 //
+// A row is read once and stays in registers until its statistics are known.  Bytes bound all of it: 16384 x 4096 bfloat16 with the
+// residual takes 91 us forward (5.9 TB/s) and 107 us back with the sum's gradient (5.0 TB/s); 4 rows 5 us, a launch and the way to memory
+// and back.
+//
 // Statistics and the quantised values are float32; s is rounded to the rows' type before its statistics are taken, because the
 // backward pass and the next layer read the rounded s.
 #include <hip/hip_runtime.h>
@@ -19,10 +23,36 @@ constexpr float kMinScale = 7.888609052210118e-31f;   // 2^-100: the scale of a 
 constexpr int kMaxNormC = 16384;
 constexpr long long kMaxGroups = (1LL << 24) - 1;   // a launch has fewer than 2^32 threads
 
+// Values c .. c + 7 of a row of C, zeros behind its end.  The last octet is loaded as the eight values that end with the row, which
+// octet() moves down once all loads are under way: element by element its lanes would wait eight times (16384 x 1500 forward 60 us,
+// so 36 us).
+template <typename T>
+__device__ __forceinline__ packed<T, 8> octet_raw(const T* row, int c, int C) {
+  if (C < 8) return load_raw<8>(row + c, C - c);
+  return load_raw<8>(row + min(c, C - 8), c < C ? 8 : 0);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x8 octet(packed<T, 8> raw, int c, int C) {
+  f32x8 v = to_floats<T, 8>(raw);
+  if (c + 8 > C && C >= 8) {
+    const int by = (8 - C % 8) & 7;   // the same for all rows
+#pragma unroll
+    for (int m = 4; m; m >>= 1)
+      if (by & m)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i + m < 8 ? v[i + m] : 0.0f;
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x8 load_octet(const T* row, int c, int C) { return octet<T>(octet_raw(row, c, C), c, C); }
+
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* sh) {
 #pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  for (int m = (LANES < 64 ? LANES : 64) / 2; m; m >>= 1) v += __shfl_xor(v, m);
   if (LANES > 64) {
     __syncthreads();   // the previous sum has been read
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
@@ -52,7 +82,8 @@ __device__ __forceinline__ float clamp_fp8(float v) {   // NaN stays NaN
 
 // The quotients are correctly rounded (an error in the last bit would move values halfway between two of the format): the reciprocal
 // is, a first correction by the exact remainder brings v r to within one unit, and a second one rounds correctly (Markstein 1990).
-// 16384 x 8192 bfloat16 takes 92 us, 4.4 TB/s; with IEEE divisions 103 us.  An exact zero loses its sign.  A remainder may lose bits below 2^-149 where a scale is near its least; that is 2^-17 of the quotient's last place at most.
+// 16384 x 8192 bfloat16 takes 92 us, 4.4 TB/s; with IEEE divisions 103 us.  An exact zero loses its sign.
+// A remainder may lose bits below 2^-149 where a scale is near its least; that is 2^-17 of the quotient's last place at most.
 struct Quotient {
   float scale, r;
   __device__ __forceinline__ explicit Quotient(float s) : scale(s), r(1.0f / s) {
@@ -99,22 +130,26 @@ rms_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, con
   __shared__ float sh[4];
   const int lane = threadIdx.x % LANES;
   const long long row = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  if (row >= rows) return;   // LANES == 256: no row is left over; LANES == 64: a wave of its own, no barrier
+  if (row >= rows) return;   // LANES == 256: no row is left over; below: the row's lanes leave together, no barrier
   const long long base = row * C;
+  packed<T, 8> raw_x[ITER], raw_r[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int c = (i * LANES + lane) * 8;
+    raw_x[i] = octet_raw(x + base, c, C);
+    if (residual) raw_r[i] = octet_raw(residual + base, c, C);
+  }
   f32x8 v[ITER];
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int c = (i * LANES + lane) * 8, n = C - c;
-    v[i] = f32x8{};
-    if (n > 0) {
-      v[i] = load8(x + base + c, n);
-      if (residual) {
-        v[i] += load8(residual + base + c, n);
+    v[i] = octet<T>(raw_x[i], c, C);
+    if (residual) {
+      v[i] += octet<T>(raw_r[i], c, C);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)v[i][j];
-        if (sum_out) store8(sum_out + base + c, v[i], n);
-      }
+      for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)v[i][j];
+      if (sum_out && n > 0) store8(sum_out + base + c, v[i], n);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
@@ -128,7 +163,7 @@ rms_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, con
     const int c = (i * LANES + lane) * 8, n = C - c;
     f32x8 o{};
     if (n > 0) {
-      const f32x8 wv = load8(w + c, n);
+      const f32x8 wv = load_octet(w, c, C);
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = v[i][j] * rstd * wv[j];
       if (y) store8(y + base + c, o, n);
@@ -143,37 +178,39 @@ rms_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, con
   }
 }
 
-// A slot is LANES threads; slot k takes rows k, k + slots, ...; its part of dw goes to part[k][C].
+// A slot is LANES threads; slot k takes rows k, k + slots, ...; a workgroup's slots add up their parts of dw, part[workgroup][C].
 template <typename T, int LANES, int ITER>
 __global__ void __launch_bounds__(256)
 rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, const float* __restrict__ w, const float* __restrict__ rstd,
-                    const T* __restrict__ d_sum, long long rows, int C, int slots, T* __restrict__ dx, float* __restrict__ part) {
+                    const T* __restrict__ d_sum, long long rows, int C, T* __restrict__ dx, float* __restrict__ part) {
   __shared__ float sh[4];
-  const int lane = threadIdx.x % LANES;
+  const int lane = threadIdx.x % LANES, slots = gridDim.x * (256 / LANES);
   const int slot = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  if (slot >= slots) return;
   f32x8 dw[ITER], wv[ITER];
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int c = (i * LANES + lane) * 8;
     dw[i] = f32x8{};
-    wv[i] = f32x8{};
-    if (c < C) wv[i] = load8(w + c, C - c);
+    wv[i] = load_octet(w, c, C);
   }
   for (long long row = slot; row < rows; row += slots) {
     const long long base = row * C;
     const float r = rstd[row];
+    packed<T, 8> raw_g[ITER], raw_h[ITER], raw_d[ITER];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * LANES + lane) * 8;
+      raw_g[i] = octet_raw(dy + base, c, C);
+      raw_h[i] = octet_raw(s + base, c, C);
+      if (d_sum) raw_d[i] = octet_raw(d_sum + base, c, C);
+    }
     f32x8 g[ITER], h[ITER];
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-      const int c = (i * LANES + lane) * 8, n = C - c;
-      g[i] = f32x8{};
-      h[i] = f32x8{};
-      if (n > 0) {
-        g[i] = load8(dy + base + c, n);
-        h[i] = load8(s + base + c, n) * r;
-      }
+      const int c = (i * LANES + lane) * 8;
+      g[i] = octet<T>(raw_g[i], c, C);
+      h[i] = octet<T>(raw_h[i], c, C) * r;
     }
 #pragma unroll
     for (int i = 0; i < ITER; ++i)
@@ -191,15 +228,31 @@ rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, const flo
         f32x8 o;
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = r * (g[i][j] - h[i][j] * dot);
-        if (d_sum) o += load8(d_sum + base + c, n);
+        if (d_sum) o += octet<T>(raw_d[i], c, C);
         store8(dx + base + c, o, n);
       }
     }
   }
+  if constexpr (LANES == 256) {
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int c = (i * LANES + lane) * 8;
-    if (c < C) store8(part + (long long)slot * C + c, dw[i], C - c);
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * LANES + lane) * 8;
+      if (c < C) store8(part + (long long)blockIdx.x * C + c, dw[i], C - c);
+    }
+  } else {
+    constexpr int kRow = LANES * 8 * ITER;
+    __shared__ float sums[256 / LANES][kRow];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[threadIdx.x / LANES][(i * LANES + lane) * 8 + j] = dw[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += 256) {
+      float v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 256 / LANES; ++k) v += sums[k][c];
+      part[(long long)blockIdx.x * C + c] = v;
+    }
   }
 }
 
@@ -219,7 +272,7 @@ quantize_fp8_kernel(const T* __restrict__ x, long long rows, int C, uint8_t* __r
   const int b = live ? (int)(blk - row * nblocks) : 0;
   const int c = b * 128 + (threadIdx.x & 15) * 8, n = C - c;
   f32x8 v{};
-  if (live && n > 0) v = load8(x + row * C + c, n);
+  if (live) v = load_octet(x + row * C, c, C);
   const float scale = block_scale(v);
   if (live && n > 0) {
     store_fp8(q + row * C + c, to_fp8(v, scale), n);
@@ -234,13 +287,17 @@ quantize_fp8_blocks_kernel(const T* __restrict__ x, int R, int C, uint8_t* __res
   __shared__ unsigned sh[4];
   const int c = blockIdx.x * 128 + (threadIdx.x & 15) * 8, n = C - c;
   const int r0 = blockIdx.y * 128 + threadIdx.x / 16;
+  packed<T, 8> raw[8];
   f32x8 v[8];
   unsigned m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + 16 * i;
-    v[i] = f32x8{};
-    if (r < R && n > 0) v[i] = load8(x + (long long)r * C + c, n);
+    raw[i] = octet_raw(x + (long long)min(r, R - 1) * C, r < R ? c : C, C);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = octet<T>(raw[i], c, C);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
   }
@@ -259,10 +316,22 @@ quantize_fp8_blocks_kernel(const T* __restrict__ x, int R, int C, uint8_t* __res
   }
 }
 
-constexpr int kMaxSlots = 1024;
+// Lanes that hold a row.  us forward and back: 65536 x 128 28 with 16 lanes, 99 with 64, 143 with 256; 16384 x 512 29 with 64, 47 with 256;
+// 16384 x 1024 54 with 64 (two octets each), 67 with 256; 16384 x 2048 131 with 64, 96 with 256.
+int norm_lanes(int C) { return C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256; }
 
-// up to four rows one slot takes them all and its part is dw: a second launch costs more than three rows one after the other
-int norm_slots(long long rows) { return rows <= 0 ? 0 : rows <= 4 ? 1 : (int)(rows < kMaxSlots ? rows : kMaxSlots); }
+// Workgroups of the backward pass, a part of dw each: as many as are on the chip at once, whose registers hold dw.  us forward and back
+// with 256 / 512 / 768 / 1024 of them: 16384 x 4096 218/202/205/212, 2000 x 8192 61/56/60/65, 2000 x 16384 123/132/139/149; one octet a
+// thread leaves room for more: 16384 x 1504 -/93/-/76.
+int norm_most_parts(int C) { return C > 8192 ? 256 : C > 1024 && C <= 2048 ? 1024 : 512; }
+
+// Up to two rows a workgroup takes them all and its part is dw: with a second launch 2 x 4096 takes about as long (8.4, 9.2 us), 4 x 4096
+// less (9.1, not 13).
+int norm_parts(long long rows, int C) {
+  const int per = 256 / norm_lanes(C);
+  const long long all = (rows + per - 1) / per;
+  return rows <= 0 ? 0 : rows <= 2 ? 1 : (int)(all < norm_most_parts(C) ? all : norm_most_parts(C));
+}
 
 template <typename T, int LANES, int ITER>
 int norm_fwd(const void* x, const void* residual, const float* w, float eps, long long rows, int C, void* sum_out, void* y, void* y8,
@@ -277,13 +346,13 @@ int norm_fwd(const void* x, const void* residual, const float* w, float eps, lon
 template <typename T, int LANES, int ITER>
 int norm_bwd(const void* dy, const void* sum, const float* w, const float* rstd, const void* d_sum, long long rows, int C, void* dx,
              float* dw, float* part, hipStream_t s) {
-  const int slots = norm_slots(rows), per = 256 / LANES;
-  if (slots == 1) part = dw;
-  if (slots > 0)
-    hipLaunchKernelGGL((rms_norm_bwd_kernel<T, LANES, ITER>), dim3((slots + per - 1) / per), dim3(256), 0, s, (const T*)dy, (const T*)sum,
-                       w, rstd, (const T*)d_sum, rows, C, slots, (T*)dx, part);
+  const int parts = norm_parts(rows, C);
+  if (parts == 1) part = dw;
+  if (parts > 0)
+    hipLaunchKernelGGL((rms_norm_bwd_kernel<T, LANES, ITER>), dim3(parts), dim3(256), 0, s, (const T*)dy, (const T*)sum, w, rstd,
+                       (const T*)d_sum, rows, C, (T*)dx, part);
   SLAMHIP_HIP(hipGetLastError());
-  if (slots != 1) SLAMHIP_HIP(column_sums(part, slots, C, WeightGradient{dw}, s));
+  if (parts != 1) SLAMHIP_HIP(column_sums(part, parts, C, WeightGradient{dw}, s));
   return SLAMHIP_OK;
 }
 
@@ -292,21 +361,24 @@ int norm_bwd(const void* dy, const void* sum, const float* w, const float* rstd,
 
 using namespace slamhip;
 
-// a row is held by one wave up to 512 values, by a workgroup of four beyond
-#define SLAMHIP_NORM_DISPATCH(FN, ...)                                                        \
-  do {                                                                                        \
-    if (dtype == SLAMHIP_BF16) {                                                              \
-      if (C <= 512) return FN<__bf16, 64, 1>(__VA_ARGS__);                                    \
-      if (C <= 2048) return FN<__bf16, 256, 1>(__VA_ARGS__);                                  \
-      if (C <= 4096) return FN<__bf16, 256, 2>(__VA_ARGS__);                                  \
-      if (C <= 8192) return FN<__bf16, 256, 4>(__VA_ARGS__);                                  \
-      return FN<__bf16, 256, 8>(__VA_ARGS__);                                                 \
-    }                                                                                         \
-    if (C <= 512) return FN<float, 64, 1>(__VA_ARGS__);                                       \
-    if (C <= 2048) return FN<float, 256, 1>(__VA_ARGS__);                                     \
-    if (C <= 4096) return FN<float, 256, 2>(__VA_ARGS__);                                     \
-    if (C <= 8192) return FN<float, 256, 4>(__VA_ARGS__);                                     \
-    return FN<float, 256, 8>(__VA_ARGS__);                                                    \
+#define SLAMHIP_NORM_LANES(FN, T, ...)                               \
+  do {                                                               \
+    switch (norm_lanes(C)) {                                         \
+      case 16: return FN<T, 16, 1>(__VA_ARGS__);                     \
+      case 32: return FN<T, 32, 1>(__VA_ARGS__);                     \
+    }                                                                \
+    if (C <= 512) return FN<T, 64, 1>(__VA_ARGS__);                  \
+    if (C <= 1024) return FN<T, 64, 2>(__VA_ARGS__);                 \
+    if (C <= 2048) return FN<T, 256, 1>(__VA_ARGS__);                \
+    if (C <= 4096) return FN<T, 256, 2>(__VA_ARGS__);                \
+    if (C <= 8192) return FN<T, 256, 4>(__VA_ARGS__);                \
+    return FN<T, 256, 8>(__VA_ARGS__);                               \
+  } while (0)
+
+#define SLAMHIP_NORM_DISPATCH(FN, ...)                               \
+  do {                                                               \
+    if (dtype == SLAMHIP_BF16) SLAMHIP_NORM_LANES(FN, __bf16, __VA_ARGS__); \
+    SLAMHIP_NORM_LANES(FN, float, __VA_ARGS__);                      \
   } while (0)
 
 extern "C" {
@@ -326,7 +398,8 @@ int slamhip_rms_norm_fwd(const void* x, const void* residual, const float* weigh
 
 size_t slamhip_rms_norm_bwd_workspace_bytes(long long rows, int C) {
   if (rows <= 0 || C <= 0) return 0;
-  return norm_slots(rows) == 1 ? 0 : (size_t)norm_slots(rows) * (size_t)C * sizeof(float);
+  const int parts = norm_parts(rows, C);
+  return parts == 1 ? 0 : (size_t)parts * (size_t)C * sizeof(float);
 }
 
 int slamhip_rms_norm_bwd(const void* dy, const void* sum, const float* weight, const float* rstd, const void* d_sum, long long rows,

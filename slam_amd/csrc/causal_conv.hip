@@ -4,7 +4,8 @@
 //   backward: d = dy silu'(pre),  dxp[p] = sum_k w[k] d[p-k],  dw[c,k] = sum d[t] xp[t+k],  dbias = sum d
 //
 // A thread walks a few channels down a run of time steps with the last K rows in registers, so a row is read from memory
-// once but for the K - 1 rows in front of a run (and, backward, as many behind it).  Nothing but the bytes bounds this.
+// once but for the K - 1 rows in front of a run (and, backward, as many behind it).  Bytes bound this: 8 x 2048 x 4096 bfloat16 takes
+// 55 us forward (268 MB, 4.9 TB/s) and 97 us back (403 MB, 4.2 TB/s), 32 x 1 x 4096 with its states 5 us: a launch and two ways to memory.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -24,8 +25,12 @@ struct ConvArgs {
   int lx_log2;   // a workgroup is 2^lx_log2 threads along the channels by 256 / 2^lx_log2 runs
 };
 
+// A thread's channels c .. c + V - 1 and steps from t0.  Where the row ends inside them they are the V that end with it, so that every
+// load is one of V, and the first `skip` belong to the thread in front: worked on and not stored (element by element a row of 1021 is
+// waited for several times: 8 x 2048 x 1021 forward and back 105 us, so 56).  n: how many there are (C < V).
 struct Place {
-  int c, n, run, t0;
+  int c, n, skip, run, t0;
+  bool live;
 };
 
 template <int V>
@@ -33,10 +38,28 @@ __device__ __forceinline__ Place conv_place(const ConvArgs& a) {
   const int lx = 1 << a.lx_log2;
   Place p;
   p.c = (blockIdx.x * lx + (threadIdx.x & (lx - 1))) * V;
+  p.live = p.c < a.C;
+  p.skip = 0;
+  if (a.C >= V && p.c > a.C - V) {
+    p.skip = p.c - (a.C - V);
+    p.c = a.C - V;
+  }
   p.n = a.C - p.c;
   p.run = blockIdx.y * (256 >> a.lx_log2) + (threadIdx.x >> a.lx_log2);
   p.t0 = p.run * a.run;
+  p.live = p.live && p.run < a.runs;
   return p;
+}
+
+template <int V, typename T>
+__device__ __forceinline__ void put(T* to, floats<V> v, const Place& p) {
+  if (p.skip == 0) {
+    storev<V>(to, v, p.n);
+  } else {
+#pragma unroll
+    for (int i = 1; i < V; ++i)
+      if (i >= p.skip) to[i] = (T)v[i];
+  }
 }
 
 __device__ __forceinline__ int conv_length(const ConvArgs& a, int b) {
@@ -70,7 +93,7 @@ template <typename T, int K, int V>
 __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
   const Place p = conv_place<V>(a);
   const int b = blockIdx.z, len = conv_length(a, b);
-  if (p.n <= 0 || p.run >= a.runs) return;
+  if (!p.live) return;
   const T* x = (const T*)a.x + b * a.xb;
   T* y = (T*)a.y + b * a.yb;
   const T* state = a.state_in ? (const T*)a.state_in + (long long)b * (K - 1) * a.C : nullptr;
@@ -87,7 +110,7 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
 #pragma unroll
       for (int k = 0; k < K - 1; ++k)
         if (len + i == k) v = win[k];
-      storev<V>(out + (long long)i * a.C + p.c, v, p.n);
+      put<V>(out + (long long)i * a.C + p.c, v, p);
     }
   }
   const int t1 = min(p.t0 + a.run, a.T), last = min(t1, len);
@@ -114,7 +137,7 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] *= sigmoid_(v[j]);
       if (t + i >= len) v = floats<V>{};
-      if (t + i < t1) storev<V>(y + (t + i) * a.yt + p.c, v, p.n);
+      if (t + i < t1) put<V>(y + (t + i) * a.yt + p.c, v, p);
 #pragma unroll
       for (int k = 0; k < K - 1; ++k) win[k] = win[k + 1];
     }
@@ -128,11 +151,10 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
   __shared__ float sh[256 * V];
   const Place p = conv_place<V>(a);
   const int b = blockIdx.z, len = conv_length(a, b);
-  const bool live = p.n > 0 && p.run < a.runs;
   floats<V> dw[K], db{};
 #pragma unroll
   for (int k = 0; k < K; ++k) dw[k] = floats<V>{};
-  if (live) {
+  if (p.live) {
     const T* x = (const T*)a.x + b * a.xb;
     const T* dy = (const T*)a.dy + b * a.dyb;
     T* dx = (T*)a.dx + b * a.dxb;
@@ -204,9 +226,9 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
             if (d_out && i_state >= 0 && i_state < K - 1) v += loadv<V>(d_out + (long long)i_state * a.C + p.c, p.n);
             if (row >= 0) {
               if (row >= len) v = floats<V>{};
-              storev<V>(dx + row * a.dxt + p.c, v, p.n);
+              put<V>(dx + row * a.dxt + p.c, v, p);
             } else if (d_in) {
-              storev<V>(d_in + (long long)(row + K - 1) * a.C + p.c, v, p.n);
+              put<V>(d_in + (long long)(row + K - 1) * a.C + p.c, v, p);
             }
           }
 #pragma unroll
@@ -226,7 +248,8 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
     const floats<V> v = k < K ? dw[k < K ? k : 0] : db;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < V; ++j) sh[j * 256 + threadIdx.x] = v[j];
+    for (int j = 0; j < V; ++j)
+      if (j >= p.skip) sh[(j - p.skip) * 256 + threadIdx.x] = v[j];
     __syncthreads();
     for (int i = threadIdx.x; i < lx * V; i += 256) {   // i = channel within the workgroup's
       float s = 0.0f;
@@ -243,7 +266,9 @@ struct ConvShape {
 
 constexpr int kChannels = 4;   // a thread's; eight take 146 and 209 registers: 67 and 206 us where four take 55 and 103
 
-// Runs are as long as leaves `waves` waves (fewer rows are read twice); short sequences take shorter ones.
+// Runs are as long as leaves `waves` waves (fewer rows are read twice); short sequences take shorter ones.  8 x 2048 x 4096 forward
+// (forward and back) with runs of at most 8 (32) 57 (160) us, 16 (64) 55 (151), 32 (128) 56 (154); 1 x 8192 x 4096 forward and back with half
+// the waves 95 us, these 85, twice 89.
 ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int waves) {
   ConvShape s;
   const int across = (C + V - 1) / V;

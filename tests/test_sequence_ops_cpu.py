@@ -147,3 +147,21 @@ def test_workspaces_of_empty_calls():
         assert lib.slamhip_selective_scan_fwd_workspace_bytes(B, T, 5, 16) == 0
         # the state's gradient passes through and the parameters' are zero: a sum for each sequence
         assert lib.slamhip_selective_scan_bwd_workspace_bytes(B, T, 5, 16) == (0 if B == 0 else B * 5 * 18 * 4)
+
+
+def test_the_binding_refuses_what_is_no_gpu_tensor():
+    m, w = torch.zeros(2, 8), torch.zeros(8)
+    s = torch.zeros(1, 3, 8)
+    with pytest.raises(ValueError, match="x: expected .*GPU matrix.*got float"):
+        ops.rms_norm_fwd(m, w, 1e-5, y=m)
+    with pytest.raises(ValueError, match="x: expected a tensor, got list"):
+        ops.rms_norm_fwd([1.0], w, 1e-5)
+    with pytest.raises(ValueError, match="sum: expected .* got None"):
+        ops.rms_norm_bwd(m, None, w, w, m, w)
+    for call in (lambda: ops.quantize_fp8(m, m, m), lambda: ops.quantize_fp8_blocks(m, m, m), lambda: ops.gemm_nt_fp8(m, m, m, m, m),
+                 lambda: ops.causal_conv_fwd(s, m, w, s), lambda: ops.causal_conv_bwd(s, s, m, w, s, m),
+                 lambda: ops.selective_scan_fwd(s, s, m, s, s, s), lambda: ops.selective_scan_bwd(s, s, s, m, s, s, w, s, s, m, s, s)):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+    with pytest.raises(TypeError, match="takes 3 arguments"):
+        ops._sequence.quantize_fp8(m)

@@ -293,8 +293,12 @@ GemmPlan gemm_plan(int M, int N, int K) {
   else if (tiles(128, 128) > 128) pick(GemmPlan::k128KW, tiles(128, 128));
   else if (tiles(64, 128) > 128) pick(GemmPlan::k64x128KW, tiles(64, 128));
   else pick(GemmPlan::k64KW, tiles(64, 64));
-  const int KB = (K + 127) / 128, least = 32;   // blocks of k that are worth a part of their own, and a launch more
-  long long parts = 256 / g.groups;
+  // Blocks of k that are worth a part of their own, and a launch more.  us with at least 8 / 12 / 16 / 32 of them: 40x478x7328 8.4/9.7/10.2/16.2,
+  // 276x490x10512 14.3/14.2/14.7/20.4, 100x500x16384 13.5/12.1/12.1/14.3, 871x562x3152 13.6/13.6/12.3/12.4; few rows, whose weights
+  // are read by more waves, 4x2048x4096 6.7/6.8/6.8/5.5.
+  const int KB = (K + 127) / 128, least = g.kind == GemmPlan::kRows ? 32 : 12;
+  // a workgroup for each CU at most, of each XCD's 32 too: with 33 112x2598x12000 takes 27 us, with fewer parts 22
+  long long parts = g.kind == GemmPlan::kRows ? 256 / g.groups : 32 / ((g.groups + 7) / 8);
   if (parts > KB / least) parts = KB / least;
   if (parts < 1) parts = 1;
   g.per = (int)(((KB + parts - 1) / parts + 3) / 4 * 4);

@@ -10,7 +10,7 @@
 // is 16 channels.  What is needed once a step and channel (softplus, gates, stores) is done by lane k of the quad for
 // steps k, k + 4, ... and handed on with quad permutes.  B_t and C_t are staged in shared memory in float32 for the workgroup's
 // 64 channels.  Vector instructions bound it: an exponential (two issue slots), two products and two multiply-adds for every (step, channel,
-// state), and once a step and channel softplus, gate, sums over the quad.  At 8 x 2048 x 2048 x 16 bfloat16 the passes of 104 and 180 us
+// state), and once a step and channel softplus, gate, sums over the quad.  At 8 x 2048 x 2048 x 16 bfloat16 the passes of 99 and 180 us
 // forward issue 23 and 34 vector instructions a step of a wave (16 and 20 of them the recurrence) and keep the units busy 81 and 84 % of
 // the time; those of 108 and 495 us back 24 and 101, 83 %.  The bytes alone would take 153 us.
 // A long sequence is cut into chunks where there are too few channels to fill the chip: a first pass leaves each chunk's own end
@@ -76,7 +76,7 @@ __device__ __forceinline__ float softplus_(float v, float e) {
 
 struct Lane {
   int q, c, cc, len, own, b;   // own: the lane's own length, 0 without a channel
-  bool live, whole;            // whole: all channels of the workgroup are there
+  bool live;
 };
 
 __device__ __forceinline__ Lane scan_lane(const ScanArgs& a) {
@@ -84,7 +84,7 @@ __device__ __forceinline__ Lane scan_lane(const ScanArgs& a) {
   l.q = threadIdx.x & 3;
   l.c = blockIdx.x * 64 + (threadIdx.x >> 2);
   l.live = l.c < a.C;
-  l.cc = l.live ? l.c : a.C - 1;   // lanes without a channel read the last one's parameters and have no steps
+  l.cc = l.live ? l.c : a.C - 1;   // lanes without a channel read the last one's values, have steps of no length and store nothing
   l.b = blockIdx.z;
   l.len = a.T;
   if (a.lengths) {
@@ -92,7 +92,6 @@ __device__ __forceinline__ Lane scan_lane(const ScanArgs& a) {
     l.len = n < 0 ? 0 : (n > a.T ? a.T : n);
   }
   l.own = l.live ? l.len : 0;
-  l.whole = (blockIdx.x + 1) * 64 <= (unsigned)a.C;
   return l;
 }
 
@@ -219,7 +218,7 @@ __global__ void __launch_bounds__(256, 4) selective_scan_fwd_kernel(ScanArgs a) 
   } else if (chunk == 0) {
     load_states<P>(a.ends + ((long long)l.b * slots * a.C + l.cc) * a.N, a.N, l.q, h);
   } else {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < chunk; ++j) {
       const float s = a.sums[((long long)l.b * a.chunks + j) * a.C + l.cc];
       float e[P];
@@ -239,7 +238,7 @@ __global__ void __launch_bounds__(256, 4) selective_scan_fwd_kernel(ScanArgs a) 
   const long long kept_step = (long long)a.C * a.N;
   T nu[G], nd[G], nz[G];
   auto fetch = [&](int t0) {
-    const bool full = l.whole && t0 + TB <= l.len;
+    const bool full = t0 + TB <= l.len;
     next_bc.load(t0, l.len);
     ru.load(nu, full, t0, l);
     rd.load(nd, full, t0, l);
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(256, 4) selective_scan_fwd_kernel(ScanArgs a) 
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         if (!STATES && i % (TK / 4) == 0 && a.kept) {
-          if (WHOLE || (l.live && t0 + 4 * i < a.T)) store_states<P>(kept, a.N, l.q, h);
+          if (l.live && (WHOLE || t0 + 4 * i < a.T)) store_states<P>(kept, a.N, l.q, h);
           kept += kept_step;
         }
         float inner[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -303,11 +302,11 @@ __global__ void __launch_bounds__(256, 4) selective_scan_fwd_kernel(ScanArgs a) 
           float v = fmaf(D, u[i], quad_sum_own(inner, l.q));
           if (Z) v *= z[i] * sigmoid_(z[i]);
           if (!WHOLE && t >= l.len) v = 0.0f;
-          if (WHOLE || (l.live && t < t_end)) ry.store(i, v);
+          if (l.live && (WHOLE || t < t_end)) ry.store(i, v);
         }
       }
     };
-    if (l.whole && t0 + TB <= l.len)
+    if (t0 + TB <= l.len)
       block(std::true_type{});
     else
       block(std::false_type{});
@@ -418,7 +417,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
   if (!CARRY || chunk == a.chunks - 1)
     if (a.d_state_out) load_states<P>(a.d_state_out + bC * a.N, a.N, l.q, g);
   if (!CARRY)
-#pragma unroll 4
+#pragma unroll 8
     for (int j = a.chunks - 1; j > chunk; --j) {   // the last chunk's own carry holds d_state_out already
       const float s = a.sums[((long long)l.b * a.chunks + j) * a.C + l.cc];
       float e[P];
@@ -448,7 +447,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
   T nu[G], nd[G], nz[G], ny[G];
   float nh[P];
   auto fetch = [&](int t0) {
-    const bool full = l.whole && t0 + TB <= l.len;
+    const bool full = t0 + TB <= l.len;
     next_bc.load(t0, l.len);
     if (!CARRY) {
       load_states<P>(kept, a.N, l.q, nh);
@@ -493,7 +492,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
     for (int i = 0; i < G; ++i) {   // behind the sequence u, dy and z are zero
       if (t0 + 4 * i + l.q >= l.own) dt[i] = 0.0f;
       if (!CARRY) u[i] = (float)nu[i];
-      e[i] = dy[i] = (float)ny[i];
+      e[i] = dy[i] = CARRY || l.live ? (float)ny[i] : 0.0f;   // the sums over the channels take no part of a lane without one
       if (CARRY) dt_sum += dt[i];
     }
     if (Z)
@@ -607,7 +606,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
           if (!in) du = dd = 0.0f;
           dD = fmaf(e[i], u[i], dD);
           dbias += dd;
-          const bool there = WHOLE || (l.live && t < t_end);
+          const bool there = l.live && (WHOLE || t < t_end);
           if (there) {
             rdu.store(i, du);
             rdd.store(i, dd);
@@ -620,7 +619,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
           }
         }
       };
-      if (l.whole && t0 + TB <= l.len)
+      if (t0 + TB <= l.len)
         reverse(std::true_type{});
       else
         reverse(std::false_type{});

@@ -491,8 +491,9 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
 #pragma unroll
     for (int i = 0; i < G; ++i) {   // behind the sequence u, dy and z are zero
       if (t0 + 4 * i + l.q >= l.own) dt[i] = 0.0f;
-      if (!CARRY) u[i] = (float)nu[i];
-      e[i] = dy[i] = CARRY || l.live ? (float)ny[i] : 0.0f;   // the sums over the channels take no part of a lane without one
+      // the sums over the channels take no part of a lane without one
+      if (!CARRY) u[i] = l.live ? (float)nu[i] : 0.0f;
+      e[i] = dy[i] = CARRY || l.live ? (float)ny[i] : 0.0f;
       if (CARRY) dt_sum += dt[i];
     }
     if (Z)

@@ -64,8 +64,8 @@ def causal_conv_fwd(x, weight, bias, y, state_in=None, state_out=None, lengths=N
     """Convolution over time of x [B, T, C] with one filter a channel, weight [C, K], 2 <= K <= 4:
     pre[t] = bias + sum_k weight[:, k] xp[t + k] with xp = state_in [B, K - 1, C] (None: zeros) followed by x, and
     y = pre * sigmoid(pre) (pre with silu=False).  state_out receives the last K - 1 rows of xp, to be state_in of the call that
-    continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths (int32 [B]) bounds each sequence:
-    rows behind it are not used and are zero in y.  x and y may be views with any strides over B and T."""
+    continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths (int32 [B], taken into [0, T]) bounds each
+    sequence: rows behind it are not used and are zero in y.  x and y may be views with any strides over B and T."""
     _sequence.causal_conv_fwd(x, weight, bias, y, state_in, state_out, lengths, silu)
 
 
@@ -87,8 +87,9 @@ def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, 
     u, delta, z, y [B, T, C], A [C, N], Bm, Cm [B, T, N], N <= 32.  D and delta_bias [C] and the gate z are optional; softplus=False
     takes delta + delta_bias as it is.  state_in [B, C, N] (None: zeros) is h before the first step and state_out h after the last,
     to be state_in of the call that continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths
-    (int32 [B]) bounds each sequence: rows behind it are not used and are zero in y.  kept_states (selective_scan_kept_states)
-    is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T."""
+    (int32 [B], taken into [0, T]) bounds each sequence: rows behind it are not used and are zero in y.  kept_states (selective_scan_kept_states)
+    is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T.  States grow where A is positive:
+    exp(A sum dt) over up to a few hundred steps has to be a float32."""
     _sequence.selective_scan_fwd(u, delta, A, Bm, Cm, y, D, z, delta_bias, softplus, state_in, state_out, kept_states, lengths)
 
 

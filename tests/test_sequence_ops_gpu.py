@@ -33,7 +33,9 @@ def rand(g, *shape, dtype=F32, scale=1.0):
 
 
 # ------------------------------------------------------------------------------------------------------------ rms norm
-NORM_SHAPES = [(1, 1), (3, 7), (5, 64), (2, 512), (7, 513), (4, 1000), (3, 2048), (2, 2049), (3, 4096), (2, 5001), (1, 8192), (2, 16384), (1500, 96)]
+NORM_SHAPES = [(1, 1), (3, 7), (5, 64), (2, 512), (7, 513), (4, 1000), (3, 2048), (2, 2049), (3, 4096), (2, 5001), (1, 8192), (2, 16384), (1500, 96),
+               # lanes for narrow rows, and more rows than the backward pass has places for
+               (40, 130), (701, 200), (5, 256), (9000, 24), (2100, 300), (1100, 1100), (600, 2100), (300, 9001)]
 
 
 @pytest.mark.parametrize("rows,C", NORM_SHAPES)
@@ -182,7 +184,7 @@ GEMM_SHAPES = [(1, 1, 16), (1, 16, 128), (3, 130, 272), (16, 64, 4096), (17, 48,
                # one for each tile shape, with odd edges: 64 x 128, 128 x 128 in two groups and in one, 256 x 256; 3, 5 and 9 blocks of k
                (700, 1500, 384), (1500, 1400, 272), (2100, 2050, 640), (3500, 3400, 1152),
                # few tiles and much k: parts of k, of which the last is short
-               (5, 40, 8336), (100, 70, 9232), (300, 200, 12304)]
+               (5, 40, 8336), (100, 70, 9232), (300, 200, 12304), (40, 478, 7328), (112, 1300, 2576)]
 
 
 def gemm_bound(av, bv):
@@ -252,7 +254,7 @@ def padded(g, B, T, C, dtype, kind, fill=NAN):
 
 
 CONV_CASES = [(1, 1, 1, 2, 0), (2, 1, 8, 4, 0), (3, 2, 5, 3, 1), (1, 3, 64, 4, 0), (2, 17, 9, 4, 2), (4, 40, 33, 3, 1), (1, 200, 136, 4, 0), (3, 65, 512, 2, 2),
-              (2, 131, 1000, 4, 1)]
+              (2, 131, 1000, 4, 1), (2, 70, 6, 3, 1), (2, 21, 1027, 4, 0), (3, 19, 270, 3, 1), (1, 9, 3, 4, 1)]
 
 
 @pytest.mark.parametrize("B,T,C,K,kind", CONV_CASES)
@@ -295,10 +297,11 @@ def test_causal_conv_forward_and_gradients(B, T, C, K, kind, dtype, state, ragge
         close(db, zero(bl.grad, bl), bound["dbias"], "dbias")
 
 
+@pytest.mark.parametrize("C", [72, 73, 75, 2])
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_causal_conv_continues_sequences(dtype):
+def test_causal_conv_continues_sequences(dtype, C):
     """One call over all steps, and calls over pieces (one step at a time at the end) with the state kept in place."""
-    B, T, C, K = 3, 37, 72, 4
+    B, T, K = 3, 37, 4
     g = torch.Generator().manual_seed(5)
     x, w, b = rand(g, B, T, C, dtype=dtype).to(DEV), rand(g, C, K).to(DEV), rand(g, C).to(DEV)
     whole = torch.empty_like(x)
@@ -857,3 +860,93 @@ def test_offsets_beyond_32_bits():
     ops.gemm_nt_fp8(a8, sa, a8, sb, out)
     ops.gemm_nt_fp8(a8[-64:].contiguous(), sa[-64:].contiguous(), a8, sb, last)
     assert torch.equal(out[-64:], last)
+
+
+# ------------------------------------------------------------------------------------------------- views and other threads
+def test_broadcast_inputs_and_their_gradients():
+    """Inputs expanded over sequences and steps (strides of zero): the gradients are those of their copies, each element's own."""
+    g = torch.Generator().manual_seed(77)
+    B, T, C, N, K = 3, 50, 70, 16, 4
+    t = scan_case(g, B, T, C, N, F32, use_z=False, state=True)
+    flat = dict(t)
+    for k, shape in (("u", (1, 1, C)), ("delta", (1, T, C)), ("Bm", (B, 1, N)), ("Cm", (1, 1, N)), ("dy", (1, T, C))):
+        one = rand(g, *shape).to(DEV)
+        t[k] = one.expand(B, T, shape[2])
+        flat[k] = t[k].contiguous()
+    want, got = scan_run(flat, F32), scan_run(t, F32)
+    for k, v in want.items():
+        assert torch.equal(got[k], v), k
+    w, b = rand(g, C, K).to(DEV), rand(g, C).to(DEV)
+    new = lambda *s: torch.full(s, NAN, device=DEV)  # noqa: E731
+    outs = []
+    for v in (flat, t):
+        y, dx, dw, db = new(B, T, C), new(B, T, C), new(C, K), new(C)
+        ops.causal_conv_fwd(v["u"], w, b, y)
+        ops.causal_conv_bwd(v["dy"], v["u"], w, b, dx, dw, db)
+        outs.append((y, dx, dw, db))
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+@pytest.mark.parametrize("C,N", [(5, 3), (70, 16), (67, 20)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_what_lies_beside_the_outputs_stays(C, N, dtype):
+    g = torch.Generator().manual_seed(C)
+    B, T, K = 2, 37, 3
+    t = scan_case(g, B, T, C, N, dtype, state=True, ragged=True)
+    c = lambda k: t[k].to(DEV)  # noqa: E731
+
+    def beside(W):
+        wide = torch.full((B + 1, T + 2, W + 5), 7.0, dtype=dtype, device=DEV)
+        return wide, wide[:B, 1:T + 1, 2:W + 2]
+
+    def untouched(wide, W):
+        wide = wide.clone()
+        inner = wide[:B, 1:T + 1, 2:W + 2]
+        assert not bool((inner == 7.0).all())
+        inner.fill_(7.0)
+        assert bool((wide == 7.0).all())
+
+    made = {k: beside(W) for k, W in (("y", C), ("du", C), ("ddelta", C), ("dz", C), ("dB", N), ("dC", N), ("cy", C), ("cdx", C))}
+    out = {k: v[1] for k, v in made.items()}
+    kept = ops.selective_scan_kept_states(B, T, C, N, DEV)
+    ops.selective_scan_fwd(t["u"], t["delta"], c("A"), t["Bm"], t["Cm"], out["y"], D=c("D"), z=t["z"], delta_bias=c("delta_bias"),
+                           kept_states=kept, lengths=c("lengths"))
+    dA = torch.empty(C, N, device=DEV)
+    ops.selective_scan_bwd(t["dy"], t["u"], t["delta"], c("A"), t["Bm"], t["Cm"], kept, out["du"], out["ddelta"], dA, out["dB"], out["dC"],
+                           D=c("D"), z=t["z"], delta_bias=c("delta_bias"), dz=out["dz"], lengths=c("lengths"))
+    w = rand(g, C, K).to(DEV)
+    dw = torch.empty_like(w)
+    ops.causal_conv_fwd(t["u"], w, None, out["cy"], lengths=c("lengths"))
+    ops.causal_conv_bwd(t["dy"], t["u"], w, None, out["cdx"], dw, lengths=c("lengths"))
+    for k, (wide, view) in made.items():
+        untouched(wide, view.shape[2])
+        for i in range(B):
+            assert not bool(view[i, int(t["lengths"][i]):].any()), k
+
+
+def test_calls_from_two_threads():
+    """Two threads, each with its own stream and operands, without waiting for each other: bits of the calls one by one."""
+    import threading
+    g = torch.Generator().manual_seed(13)
+    sets = [scan_case(g, 2, 300, 48, 16, F32, state=True) for _ in range(2)]
+    want = [scan_run(t, F32) for t in sets]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got = scan_run(sets[i], F32)
+                    stream.synchronize()
+                    assert all(torch.equal(got[k], v) for k, v in want[i].items())
+        except BaseException as e:  # noqa: B902
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

@@ -221,10 +221,11 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
 }
 
 // Up to 16 rows: the weights are read once, straight into registers (one fragment serves all rows); a workgroup's waves take every
-// eighth block of k for the same 16 columns and meet in shared memory.  U blocks are under way at once, all of K = 4096.  Bound by
-// the weights' bytes: 4 x 8192 x 4096 takes 9.5 us, 3.5 TB/s.  From 17 rows on the tiles are faster (12 against 18 us at 32 rows).
-__global__ void __launch_bounds__(512) gemm_fp8_rows_kernel(GemmArgs p) {
-  constexpr int kWaves = 8, U = 4;
+// 16th block of k for the same 16 columns and meet in shared memory.  U blocks of a wave are under way at once, all of K = 4096.  Bound by
+// the weights' bytes: 4 x 16384 x 4096 takes 15.3 us, 4.4 TB/s (8 waves and four blocks 16.6), 4 x 8192 x 4096 9.5 us (9.9).  From 17 rows on
+// the tiles are faster (12 against 18 us at 32 rows).
+__global__ void __launch_bounds__(1024) gemm_fp8_rows_kernel(GemmArgs p) {
+  constexpr int kWaves = 16, U = 2;
   __shared__ f32x4 sh[kWaves][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n0 = blockIdx.x * 16, row = lane & 15, g = lane >> 4;
@@ -314,7 +315,7 @@ void gemm_tiles(const GemmArgs& p, const GemmPlan& g, hipStream_t s) {
 int gemm(const GemmArgs& p, const GemmPlan& g, hipStream_t s) {
   const dim3 rows((unsigned)g.groups, g.parts);
   switch (g.kind) {
-    case GemmPlan::kRows: hipLaunchKernelGGL(gemm_fp8_rows_kernel, rows, dim3(512), 0, s, p); break;
+    case GemmPlan::kRows: hipLaunchKernelGGL(gemm_fp8_rows_kernel, rows, dim3(1024), 0, s, p); break;
     case GemmPlan::k256: gemm_tiles<256, 256, 2, 4, 2, 1>(p, g, s); break;
     case GemmPlan::k128: gemm_tiles<128, 128, 2, 2, 2, 1>(p, g, s); break;
     case GemmPlan::k128KW: gemm_tiles<128, 128, 2, 2, 2, 2>(p, g, s); break;

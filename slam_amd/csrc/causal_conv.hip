@@ -68,11 +68,11 @@ __device__ __forceinline__ int conv_length(const ConvArgs& a, int b) {
   return n < 0 ? 0 : (n > a.T ? a.T : n);
 }
 
-// row `t` of a sequence: state rows in front of it, zeros where it has neither
+// row `t` of a sequence as it is in memory: state rows in front of it, zeros where it has neither
 template <typename T, int K, int V>
-__device__ __forceinline__ floats<V> conv_row(const ConvArgs& a, const T* x, const T* state, int t, int len, int c, int n) {
-  if (t >= 0) return t < len ? loadv<V>(x + t * a.xt + c, n) : floats<V>{};
-  return state ? loadv<V>(state + (long long)(t + K - 1) * a.C + c, n) : floats<V>{};
+__device__ __forceinline__ packed<T, V> conv_row(const ConvArgs& a, const T* x, const T* state, int t, int len, int c, int n) {
+  const T* from = t >= 0 ? x + t * a.xt : state + (long long)(t + K - 1) * a.C;
+  return load_raw<V>(from + c, t >= 0 ? (t < len ? n : 0) : (state ? n : 0));
 }
 
 // a thread's filters lie one behind the other: V K floats
@@ -97,22 +97,18 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
   const T* x = (const T*)a.x + b * a.xb;
   T* y = (T*)a.y + b * a.yb;
   const T* state = a.state_in ? (const T*)a.state_in + (long long)b * (K - 1) * a.C : nullptr;
+  // all loads that a run begins with are under way before the first is converted
+  packed<T, V> front[K - 1], left[K - 1];
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) front[k] = conv_row<T, K, V>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
+  const bool leaves = p.run == 0 && a.state_out;
+#pragma unroll
+  for (int i = 0; i < K - 1; ++i) {
+    const int t = len + i - (K - 1);
+    left[i] = load_raw<V>(x + (t > 0 ? t : 0) * a.xt + p.c, leaves && t >= 0 ? p.n : 0);
+  }
   floats<V> w[K], bias, win[K];
   conv_weights<K, V>(a, p.c, p.n, w, bias);
-#pragma unroll
-  for (int k = 0; k < K - 1; ++k) win[k] = conv_row<T, K, V>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
-  if (p.run == 0 && a.state_out) {   // win holds the state: it may be written over from here on
-    T* out = (T*)a.state_out + (long long)b * (K - 1) * a.C;
-#pragma unroll
-    for (int i = 0; i < K - 1; ++i) {
-      floats<V> v{};
-      if (len + i >= K - 1) v = loadv<V>(x + (len + i - (K - 1)) * a.xt + p.c, p.n);
-#pragma unroll
-      for (int k = 0; k < K - 1; ++k)
-        if (len + i == k) v = win[k];
-      put<V>(out + (long long)i * a.C + p.c, v, p);
-    }
-  }
   const int t1 = min(p.t0 + a.run, a.T), last = min(t1, len);
   packed<T, V> next[4];
   auto fetch = [&](int t) {
@@ -120,6 +116,19 @@ __global__ void __launch_bounds__(256) causal_conv_fwd_kernel(ConvArgs a) {
     for (int i = 0; i < 4; ++i) next[i] = load_raw<V>(x + (t + i) * a.xt + p.c, t + i < last ? p.n : 0);
   };
   fetch(p.t0);
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) win[k] = to_floats<T, V>(front[k]);
+  if (leaves) {   // win holds the state: it may be written over from here on
+    T* out = (T*)a.state_out + (long long)b * (K - 1) * a.C;
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) {
+      floats<V> v = to_floats<T, V>(left[i]);
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+        if (len + i == k) v = win[k];
+      put<V>(out + (long long)i * a.C + p.c, v, p);
+    }
+  }
   for (int t = p.t0; t < t1; t += 4) {
     packed<T, V> now[4];
 #pragma unroll
@@ -162,13 +171,11 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
     const T* state = a.state_in ? (const T*)a.state_in + sbase : nullptr;
     const T* d_out = a.d_state_out ? (const T*)a.d_state_out + sbase : nullptr;
     T* d_in = a.d_state_in ? (T*)a.d_state_in + sbase : nullptr;
+    packed<T, V> front[K - 1];
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) front[k] = conv_row<T, K, V>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
     floats<V> w[K], bias, win[K], d[K];
     conv_weights<K, V>(a, p.c, p.n, w, bias);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      d[k] = floats<V>{};   // d[k] is the gradient at pre of step t - (K - 1) + k
-      if (k < K - 1) win[k] = conv_row<T, K, V>(a, x, state, p.t0 + k - (K - 1), len, p.c, p.n);
-    }
     const int t1 = min(p.t0 + a.run, a.T);
     const int first = p.run == 0 ? -(K - 1) : p.t0;   // the first run's rows begin with the state's
     const int last = min(t1 + K - 1, len);
@@ -181,6 +188,11 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
       }
     };
     fetch(p.t0);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      d[k] = floats<V>{};   // d[k] is the gradient at pre of step t - (K - 1) + k
+      if (k < K - 1) win[k] = to_floats<T, V>(front[k]);
+    }
     for (int t = p.t0; t < t1 + K - 1; t += U) {
       packed<T, V> nx[U], ny[U];
 #pragma unroll
@@ -268,7 +280,7 @@ constexpr int kChannels = 4;   // a thread's; eight take 146 and 209 registers: 
 
 // Runs are as long as leaves `waves` waves (fewer rows are read twice); short sequences take shorter ones.  8 x 2048 x 4096 forward
 // (forward and back) with runs of at most 8 (32) 57 (160) us, 16 (64) 55 (151), 32 (128) 56 (154); 1 x 8192 x 4096 forward and back with half
-// the waves 95 us, these 85, twice 89.
+// the waves 95 us, these 85, twice 89.  Shortest runs of 4 rows rather than 8: 2 x 160 x 261 forward and back 21 us, not 26.
 ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int waves) {
   ConvShape s;
   const int across = (C + V - 1) / V;
@@ -287,7 +299,7 @@ ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int wav
 }
 
 ConvShape fwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 16, 4, 8192); }
-ConvShape bwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 64, 8, 4096); }
+ConvShape bwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 64, 4, 4096); }
 
 template <typename T>
 int conv_fwd(const ConvArgs& a, int K, dim3 grid, hipStream_t s) {

@@ -181,8 +181,8 @@ def test_quantize_special_values():
 # ---------------------------------------------------------------------------------------------------------- the product
 GEMM_SHAPES = [(1, 1, 16), (1, 16, 128), (3, 130, 272), (16, 64, 4096), (17, 48, 640), (33, 200, 144), (64, 16, 128), (65, 1, 16), (65, 129, 400),
                (128, 128, 128), (200, 300, 1040), (257, 513, 384), (300, 64, 2048), (777, 520, 1024),
-               # one for each tile shape, with odd edges: 64 x 128, 128 x 128 in two groups and in one, 256 x 256; 3, 5 and 9 blocks of k
-               (700, 1500, 384), (1500, 1400, 272), (2100, 2050, 640), (3500, 3400, 1152),
+               # one for each tile shape, with odd edges: 64 x 128, 128 x 128, 256 x 256; 3, 5 and 9 blocks of k; 128 x 128 in two groups
+               (700, 1500, 384), (1500, 1400, 272), (2100, 2050, 640), (3500, 3400, 1152), (1500, 1400, 2192),
                # few tiles and much k: parts of k, of which the last is short
                (5, 40, 8336), (100, 70, 9232), (300, 200, 12304), (40, 478, 7328), (112, 1300, 2576)]
 

@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include "common.h"
+#include "gemm_fp8_plan.h"
 #include "sequence_device.h"
 
 namespace slamhip {
@@ -63,8 +64,6 @@ __device__ __forceinline__ void store_out(const GemmArgs& p, int m, int n, f32x4
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
-constexpr unsigned kBeyond = 0x80000000u;   // an offset past every operand, which are smaller, also with what is added to it
-
 typedef const float __attribute__((address_space(4))) ConstFloat;
 
 // until at most N of the wave's loads are under way, and none of its reads of shared memory
@@ -84,8 +83,8 @@ __device__ __forceinline__ ConstFloat* uniform_floats(const float* p) { return (
 template <int BM, int BN, int WM, int WN, int NS, int KW>
 __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs p) {
   constexpr int kWaves = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, kLoadA = BM / 8 / kWaves, kLoadB = BN / 8 / kWaves, kLoads = kLoadA + kLoadB;
-  constexpr int kSlice = (BM + BN) * 128, kScales = BM * 16;
-  static_assert(NS >= 2 && NS <= 4 && (KW == 1 || KW == 2) && 128 % (BN / WN) == 0 && BM % 64 == 0 && BM / 64 <= kWaves, "a wave's columns share a scale");
+  constexpr int kSlice = (BM + BN) * 128, kScales = BM * 16, kLoadS = (BM / 16 + kWaves * KW - 1) / (kWaves * KW);
+  static_assert(NS >= 2 && NS <= 4 && (KW == 1 || KW == 2) && 128 % (BN / WN) == 0, "a wave's columns share a scale");
   __shared__ __align__(1024) uint8_t sh[NS * KW * kSlice + 4 * kScales];
   static_assert(KW == 1 || NS * KW * kSlice >= BM * BN * 4, "the groups' sums meet where the slices were");
   const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -102,29 +101,32 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
   const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)p.b, 0, (unsigned)((size_t)p.N * p.K), 0x00020000);
   const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)p.sa, 0, (unsigned)((size_t)p.M * p.KB * 4), 0x00020000);
 
-  // A wave's load moves 8 rows of a slice: lane l brings chunk (l & 7) ^ (row & 7) of row l >> 3.  Rows behind the last have
-  // addresses behind the operand by themselves.
+  // A wave's load moves 8 rows of a slice: lane l brings chunk (l & 7) ^ (row & 7) of row l >> 3.
   const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
-  const unsigned off_a = (unsigned)(m0 + wave * 8 + lrow) * (unsigned)p.K + lchunk * 16;
-  const unsigned off_b = (unsigned)(n0 + wave * 8 + lrow) * (unsigned)p.K + lchunk * 16;
-  const unsigned off_s = (unsigned)(m0 + wave * 64 + lane) * (unsigned)p.KB * 4;
+  const unsigned off_a = operand_offset(m0 + wave * 8 + lrow, lchunk, p.K), off_b = operand_offset(n0 + wave * 8 + lrow, lchunk, p.K);
   auto load = [&](int it, int buf) {
     const int kb = kb_begin + it * KW + kg;
-    const bool in = kb * 128 + lchunk * 16 < p.K;
-    const unsigned va = in ? off_a : kBeyond, vb = in ? off_b : kBeyond;
+    const unsigned block = block_offset(kb, p.KB);
     uint8_t* to = sh + (buf * KW + kg) * kSlice;
 #pragma unroll
     for (int i = 0; i < kLoadA; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(to + (i * kWaves + wave) * 1024), 16, va, kb * 128 + i * kWaves * 8 * p.K, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(to + (i * kWaves + wave) * 1024), 16, operand_load(off_a, kb, lchunk, i * kWaves * 8, p.K), block, 0, 0);
 #pragma unroll
     for (int i = 0; i < kLoadB; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(to + BM * 128 + (i * kWaves + wave) * 1024), 16, vb, kb * 128 + i * kWaves * 8 * p.K, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(to + BM * 128 + (i * kWaves + wave) * 1024), 16, operand_load(off_b, kb, lchunk, i * kWaves * 8, p.K), block, 0, 0);
   };
-  // The rows' scales come for four blocks of k at a time, 16 bytes a row: a row's scales are one after the other, and a load of one
-  // for each row touches as many lines of memory (331 instead of 299 us at 8192 x 8192 x 4096).
+  // The rows' scales come for four blocks of k at a time, 16 bytes a row: a row's scales are one after the other, and bringing one
+  // for each row and block touches four times as many lines of memory (331 instead of 299 us at 8192 x 8192 x 4096).
   uint8_t* const scales = sh + NS * KW * kSlice;
+  // A load is one float a lane, so that each is inside the rows' scales or not: 16 rows a wave.
   auto load_scales = [&](int four) {
-    if (all_waves < BM / 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(scales + (four & 3) * kScales + wave * 1024), 16, off_s, four * 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kLoadS; ++i) {
+      const int group = i * kWaves * KW + all_waves;
+      if (group < BM / 16)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(scales + (four & 3) * kScales + group * 256), 4,
+                                                 scale_load(m0 + group * 16 + (lane >> 2), four * 4 + (lane & 3), p.M, p.KB), 0, 0, 0);
+    }
   };
   const int frow = lane & 15, g = lane >> 4;
   const int c0 = frow * 128 + (g ^ (frow & 7)) * 16, c1 = frow * 128 + ((g + 4) ^ (frow & 7)) * 16;
@@ -271,42 +273,6 @@ __global__ void __launch_bounds__(256) gemm_fp8_parts_kernel(const float* __rest
 #pragma unroll 4
   for (int i = 1; i < parts; ++i) v += loadv<4>(part + i * n + at, valid);
   storev<4>(out + at, v, valid);
-}
-
-// How a product is cut: the kernel by the number of rows and tiles, and parts of k where that leaves most CUs idle.
-struct GemmPlan {
-  enum Kind { kRows, k256, k128, k128KW, k64x128KW, k64KW } kind;
-  long long groups;
-  int per, parts;
-};
-
-GemmPlan gemm_plan(int M, int N, int K) {
-  GemmPlan g;
-  auto tiles = [&](int bm, int bn) { return (long long)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  auto pick = [&](GemmPlan::Kind kind, long long groups) { g.kind = kind, g.groups = groups; };
-  // The smallest tiles while there is one for each of the 256 CUs at most (they wait least for each other), then larger ones, which read
-  // operands less often: 256^2 where k is long enough for its start and end, and two groups of waves (KW = 2) where a CU has one
-  // workgroup and k is long.  us, 256^2 / 128^2 / 128^2 KW / 64 x 128 KW / 64^2 KW: 4096x4096x4096 68/83/93/115/153, 2048x4096x4096
-  // 59/42/48/59/77, 1024x4096x4096 57/28/26/31/40, 777x2056x4096 54/25/22/16/21, 1024x1024x4096 56/25/22/16/12, 645x1434x3584
-  // 37/19/19/14/11, 306x6016x1408 28/12/13/9/13, 2225x7997x640 46/34/48/57/80, 1028x2864x896 19/9.5/10.7/14/15.
-  const int KB = (K + 127) / 128;
-  if (M <= 16) pick(GemmPlan::kRows, (N + 15) / 16);
-  else if (tiles(64, 64) <= 256) pick(GemmPlan::k64KW, tiles(64, 64));
-  else if (tiles(64, 128) <= 256) pick(GemmPlan::k64x128KW, tiles(64, 128));
-  else if (tiles(256, 256) >= 192 && KB >= 8) pick(GemmPlan::k256, tiles(256, 256));
-  else if (tiles(128, 128) <= 256 && KB > 16) pick(GemmPlan::k128KW, tiles(128, 128));
-  else pick(GemmPlan::k128, tiles(128, 128));
-  // Blocks of k that are worth a part of their own, and a launch more.  us with at least 8 / 12 / 16 / 32 of them: 40x478x7328 8.4/9.7/10.2/16.2,
-  // 276x490x10512 14.3/14.2/14.7/20.4, 100x500x16384 13.5/12.1/12.1/14.3, 871x562x3152 13.6/13.6/12.3/12.4; few rows, whose weights
-  // are read by more waves, 4x2048x4096 6.7/6.8/6.8/5.5.
-  const int least = g.kind == GemmPlan::kRows ? 32 : 12;
-  // a workgroup for each CU at most, of each XCD's 32 too: with 33 112x2598x12000 takes 27 us, with fewer parts 22
-  long long parts = g.kind == GemmPlan::kRows ? 256 / g.groups : 32 / ((g.groups + 7) / 8);
-  if (parts > KB / least) parts = KB / least;
-  if (parts < 1) parts = 1;
-  g.per = (int)(((KB + parts - 1) / parts + 3) / 4 * 4);
-  g.parts = (KB + g.per - 1) / g.per;
-  return g;
 }
 
 template <int BM, int BN, int WM, int WN, int NS, int KW>

@@ -143,3 +143,12 @@ def test_the_plan_covers_every_tile(lib):
         bm, bn = (16, 16) if kind == "rows" else TILES[kind][:2]
         assert groups == (1 if kind == "rows" else -(-M // bm)) * -(-N // bn)
         assert per % 4 == 0 and parts * per >= KB > (parts - 1) * per
+
+
+def test_the_long_products_reach_every_kind(lib):
+    """The shapes that the GPU tests take for each kind: one part of k, more blocks than the buffers of slices and of scales hold."""
+    from test_sequence_ops_long_gpu import GEMM_LONG
+    assert sorted(GEMM_LONG) == sorted(KINDS)
+    for kind, (M, N, K) in GEMM_LONG.items():
+        got, _, per, parts = plan(lib, M, N, K)
+        assert got == kind and parts == 1 and per >= 18 and K % 128, kind

@@ -704,21 +704,22 @@ struct ScanShape {
 // thirds of the second whatever their number).  Measured at 8 x 2048 steps x 2048 channels x 16 states (1024 waves): whole 271 us
 // forward and 665 us back, cut in 8 98 + 180 us and 105 + 495 us; at 1024 waves and more a short sequence stays whole (32 x 130 x
 // 700 x 4 forward 22 us, cut 25 us).  A chunk also joins all those in front of it, one after the other, so none is shorter than
-// the square root of the sequence: 1 x 4096 x 64 x 16 forward takes 83, 48, 36, 41 us in chunks of 16, 32, 64, 128, and
-// 1 x 200 x 512 x 16 takes 12, 15, 21 us in chunks of 16, 32, 64.
-ScanShape scan_shape(int B, int T, int C, int N) {
+// the square root of the sequence: 1 x 4096 x 64 x 16 forward takes 83, 48, 36, 41 us in chunks of 16, 32, 64, 128.  What is shorter than
+// two of the shortest chunks stays whole: 1 x 31 x 512 x 16 forward 6.8 us, cut 8.5.
+// Back, the shortest chunks are 16 steps longer where they make more than 2048 waves, whose sums and joins cost more than their steps: us
+// back with the shortest and the longer ones, 5 x 200 x 1000 x 8 34 and 31, 4 x 333 x 1024 x 16 50 and 44; below, 1 x 200 x 512 x 16
+// 18 and 22, 2 x 500 x 300 x 32 41 and 49.
+ScanShape scan_shape(int B, int T, int C, int N, bool back) {
   ScanShape s;
   s.P = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
   s.groups = (C + 63) / 64;
   const long long waves = (long long)(B > 0 ? B : 1) * s.groups * 4;   // without sequences the parameters' gradients are still asked for
   int shortest = 16;
   while ((long long)shortest * shortest < T) shortest += 16;
-  long long chunks = waves >= 2048 || (waves >= 1024 && T < 512) ? 1 : (8192 + waves - 1) / waves;
-  if (chunks > T / shortest) chunks = T / shortest;
-  if (chunks < 1) chunks = 1;
-  const int per = (int)((T + chunks - 1) / chunks);
-  s.chunk = (per + 15) / 16 * 16;
-  if (s.chunk < 16) s.chunk = 16;
+  const long long chunks = waves >= 2048 || (waves >= 1024 && T < 512) || T < 2 * shortest ? 1 : (8192 + waves - 1) / waves;
+  if (back && waves * ((T + shortest - 1) / shortest) > 2048) shortest += 16;
+  const int even = (int)(((T + chunks - 1) / chunks + 15) / 16 * 16);
+  s.chunk = even > shortest ? even : shortest;
   s.chunks = T > 0 ? (T + s.chunk - 1) / s.chunk : 1;
   return s;
 }
@@ -782,13 +783,13 @@ extern "C" {
 
 size_t slamhip_selective_scan_kept_floats(int B, int T, int C, int N) {
   if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
-  const int tb = kept_steps(scan_shape(B, T, C, N).P);
+  const int tb = kept_steps(scan_shape(B, T, C, N, false).P);
   return (size_t)B * ((T + tb - 1) / tb) * C * N;
 }
 
 size_t slamhip_selective_scan_fwd_workspace_bytes(int B, int T, int C, int N) {
   if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
-  const ScanShape g = scan_shape(B, T, C, N);
+  const ScanShape g = scan_shape(B, T, C, N, false);
   if (g.chunks == 1) return 0;
   return ((size_t)B * (g.chunks + 1) * C * N + (size_t)B * g.chunks * C) * sizeof(float);
 }
@@ -803,7 +804,7 @@ int slamhip_selective_scan_fwd(const void* u, const void* delta, const void* z, 
   SLAMHIP_REQUIRE(workspace_bytes >= slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N) &&
                       (workspace || slamhip_selective_scan_fwd_workspace_bytes(B, T, C, N) == 0),
                   SLAMHIP_E_ARG, "selective_scan_fwd: workspace too small");
-  const ScanShape g = scan_shape(B, T, C, N);
+  const ScanShape g = scan_shape(B, T, C, N, false);
   ScanArgs a{};
   a.u = u, a.delta = delta, a.z = z, a.Bm = Bm, a.Cm = Cm, a.A = A, a.D = D, a.bias = delta_bias, a.state_in = state_in;
   a.y = y, a.state_out = state_out, a.kept = kept_states, a.lengths = lengths;
@@ -819,7 +820,7 @@ int slamhip_selective_scan_fwd(const void* u, const void* delta, const void* z, 
 
 size_t slamhip_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N) {
   if (B <= 0 || T < 0 || C <= 0 || N <= 0 || N > 32) return 0;
-  const ScanShape g = scan_shape(B, T, C, N);
+  const ScanShape g = scan_shape(B, T, C, N, true);
   const size_t carry = g.chunks > 1 ? (size_t)B * g.chunks * C * (N + 1) : 0;
   return (carry + (size_t)B * g.chunks * C * (N + 2) + (size_t)B * T * g.groups * 8 * g.P) * sizeof(float);
 }
@@ -837,7 +838,7 @@ int slamhip_selective_scan_bwd(const void* dy, const void* u, const void* delta,
   SLAMHIP_REQUIRE(!data || !z == !dz, SLAMHIP_E_ARG, "selective_scan_bwd: z and dz come together");
   SLAMHIP_REQUIRE(workspace_bytes >= slamhip_selective_scan_bwd_workspace_bytes(B, T, C, N), SLAMHIP_E_ARG, "selective_scan_bwd: workspace too small");
   hipStream_t s = (hipStream_t)stream;
-  const ScanShape g = scan_shape(B, T, C, N);
+  const ScanShape g = scan_shape(B, T, C, N, true);
   const long long columns = (long long)C * (N + 2), bc_groups = work ? ((long long)B * T * 8 * g.P + 255) / 256 : 0;
   const long long all_groups = bc_groups + (columns + 31) / 32;
   SLAMHIP_REQUIRE(all_groups < (1 << 24) && (long long)B * g.chunks < (1 << 30), SLAMHIP_E_SIZE, "selective_scan_bwd: too many steps or parameters");

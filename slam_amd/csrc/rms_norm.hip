@@ -121,11 +121,12 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, uint2 q, int valid) {
   }
 }
 
-// LANES threads hold one row: octet i of thread t is octet i * LANES + t of the row.
+// LANES threads hold one row: octet i of thread t is octet i * LANES + t of the row.  sum_out and y may be x or residual: a thread stores
+// an octet when it has loaded it, and what another thread loads beside its own (the last octet of a row) it drops.
 template <typename T, int LANES, int ITER>
 __global__ void __launch_bounds__(256)
-rms_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const float* __restrict__ w, float eps, long long rows,
-                    int C, T* __restrict__ sum_out, T* __restrict__ y, uint8_t* __restrict__ y8, float* __restrict__ scales,
+rms_norm_fwd_kernel(const T* x, const T* residual, const float* __restrict__ w, float eps, long long rows,
+                    int C, T* sum_out, T* y, uint8_t* __restrict__ y8, float* __restrict__ scales,
                     float* __restrict__ rstd_out) {
   __shared__ float sh[4];
   const int lane = threadIdx.x % LANES;
@@ -179,10 +180,11 @@ rms_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, con
 }
 
 // A slot is LANES threads; slot k takes rows k, k + slots, ...; a workgroup's slots add up their parts of dw, part[workgroup][C].
+// dx may be dy or d_sum, whose octets are loaded before dx's is stored.
 template <typename T, int LANES, int ITER>
 __global__ void __launch_bounds__(256)
-rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, const float* __restrict__ w, const float* __restrict__ rstd,
-                    const T* __restrict__ d_sum, long long rows, int C, T* __restrict__ dx, float* __restrict__ part) {
+rms_norm_bwd_kernel(const T* dy, const T* __restrict__ s, const float* __restrict__ w, const float* __restrict__ rstd,
+                    const T* d_sum, long long rows, int C, T* dx, float* __restrict__ part) {
   __shared__ float sh[4];
   const int lane = threadIdx.x % LANES, slots = gridDim.x * (256 / LANES);
   const int slot = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;

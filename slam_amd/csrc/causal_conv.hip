@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
     conv_weights<K, V>(a, p.c, p.n, w, bias);
     const int t1 = min(p.t0 + a.run, a.T);
     const int first = p.run == 0 ? -(K - 1) : p.t0;   // the first run's rows begin with the state's
-    const int last = min(t1 + K - 1, len);
+    const int last = min(t1 + K - 1, len), mine = min(t1, len);
     packed<T, V> next_x[U], next_y[U];
     auto fetch = [&](int t) {
 #pragma unroll
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) causal_conv_bwd_kernel(ConvArgs a) {
             }
           }
           d[K - 1] = g;
-          if (now < t1) {
+          if (now < mine) {   // behind the sequence there is no product, whatever its last rows or its state hold
             db += g;
 #pragma unroll
             for (int k = 0; k < K; ++k)

@@ -567,6 +567,7 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
             read_states<P>(sh, Bv);
             read_states<P>(sh + 4 * P, Cv);
             const float d = quad_lane<K>(dt[i]), xv = quad_lane<K>(x), ev = quad_lane<K>(e[i]);
+            const bool inside = t0 + 4 * i + K < l.len;
             float s_in = 0.0f, s_gb = 0.0f, s_qa = 0.0f;
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -578,7 +579,8 @@ __global__ void __launch_bounds__(256, P == 8 && !CARRY ? 1 : 2) selective_scan_
               g[p] *= as[4 * i + K][p];
               h[p] = hs[4 * i + K][p];
               const float q = g[p] * h[p];
-              dA[p] = fmaf(q, d, dA[p]);
+              // behind the sequence d is zero, but its state (of a slot that is not used, say) may be no number
+              if (WHOLE || inside) dA[p] = fmaf(q, d, dA[p]);
               s_qa = fmaf(q, A2[p], s_qa);
             }
             // the sums are finished here: left to the end of the group they would keep B, C and the products of all four steps

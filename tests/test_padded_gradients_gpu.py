@@ -5,7 +5,7 @@ import torch
 
 from oracle import sequence_oracle as so
 from slam_amd.network import sequence_ops as ops
-from test_sequence_ops_gpu import BF16, DEV, F32, NAN, close, rand
+from test_sequence_ops_gpu import BF16, DEV, F32, NAN, close, rand, scan_case, scan_run, scan_want
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -60,3 +60,28 @@ def test_convolution_of_an_infinite_last_row(dtype, len0):
     # the last tap alone meets the last row
     assert bool(out[0][2, K - 1].isinf()) and int(out[0].isfinite().sum()) == C * K - 1
     assert torch.equal(out[0], out[1])
+
+
+@pytest.mark.parametrize("T,C,N", [(1, 5, 4), (20, 70, 3), (40, 9, 8), (150, 64, 16), (70, 30, 20)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scan_with_unused_slots(T, C, N, dtype):
+    """Sequences 1 and 3 have no rows; one has NaN in its state, the other an infinity in its state and NaN in the gradient that arrives
+    there: the gradients of all parameters and of the other sequences are those without them."""
+    g = torch.Generator().manual_seed(T + C)
+    B, keep = 4, [0, 2]
+    t = scan_case(g, B, T, C, N, dtype, state=True)
+    t["lengths"] = torch.tensor([T, 0, T // 2 + 1, 0], dtype=torch.int32)
+    few = {k: v if v is None or k in ("A", "D", "delta_bias") else v[keep] for k, v in t.items()}
+    want, bound = scan_want(few)
+    for i in range(B):
+        for name in ("u", "delta", "dy", "z", "Bm", "Cm"):
+            t[name][i, int(t["lengths"][i]):] = NAN
+    t["state_in"][1], t["state_in"][3], t["d_state_out"][3] = NAN, INF, NAN
+    got = scan_run(t, dtype)
+    for k, v in got.items():
+        close(v if k in ("dA", "dD", "d_delta_bias") else v[keep], want[k], bound[k], k)
+    for k in ("y", "du", "ddelta", "dz", "dB", "dC"):
+        assert not bool(got[k][1].any()) and not bool(got[k][3].any()), k
+    # states and their gradients pass through
+    assert bool(got["state_out"][1].isnan().all()) and bool(got["state_out"][3].isinf().all()) and bool(got["d_state_in"][3].isnan().all())
+    assert torch.equal(got["d_state_in"][1].cpu(), t["d_state_out"][1])

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW, 2) gemm_fp8_kernel(GemmArgs
   // Workgroups of one XCD (every eighth) take neighbouring tiles, eight rows of tiles at a time: they share operands in its L2.
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, total = tiles_m * tiles_n;
   const int per_xcd = (total + 7) / 8, work = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if (work >= total || (int)(blockIdx.x >> 3) >= per_xcd) return;
+  if (work >= total) return;
   const int band = work / (8 * tiles_n), high = min(8, tiles_m - band * 8), in_band = work - band * 8 * tiles_n;
   const int m0 = (band * 8 + in_band % high) * BM, n0 = in_band / high * BN;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);

@@ -75,8 +75,6 @@ __device__ __forceinline__ void storev(T* p, floats<V> v, int valid) {
 }
 
 template <typename T>
-__device__ __forceinline__ f32x8 load8(const T* p, int valid) { return loadv<8>(p, valid); }
-template <typename T>
 __device__ __forceinline__ void store8(T* p, f32x8 v, int valid) { storev<8>(p, v, valid); }
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }

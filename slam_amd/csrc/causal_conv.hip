@@ -298,6 +298,9 @@ ConvShape conv_shape(int B, int T, int C, int V, int longest, int align, int wav
   return s;
 }
 
+// the limits of the entry points; a size beyond them needs no workspace, because its call is refused
+bool conv_fits(int B, int T, int C) { return B <= 65535 && T <= (1 << 20) && C <= (1 << 20); }
+
 ConvShape fwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 16, 4, 8192); }
 ConvShape bwd_shape(int B, int T, int C) { return conv_shape(B, T, C, kChannels, 64, 4, 4096); }
 
@@ -344,7 +347,7 @@ int slamhip_causal_conv_fwd(const void* x, const long long* strides, const float
                             void* stream) {
   SLAMHIP_REQUIRE(B >= 0 && T >= 0 && C > 0 && K >= 2 && K <= 4 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG,
                   "causal_conv_fwd: need C >= 1, 2 <= K <= 4 and a known type");
-  SLAMHIP_REQUIRE(B <= 65535 && T <= (1 << 20) && C <= (1 << 20), SLAMHIP_E_SIZE, "causal_conv_fwd: at most 65535 sequences, 2^20 steps and channels");
+  SLAMHIP_REQUIRE(conv_fits(B, T, C), SLAMHIP_E_SIZE, "causal_conv_fwd: at most 65535 sequences, 2^20 steps and channels");
   if (B == 0 || (T == 0 && !state_out)) return SLAMHIP_OK;
   SLAMHIP_REQUIRE(weight && (T == 0 || (x && y && strides)), SLAMHIP_E_ARG, "causal_conv_fwd: null pointer");
   ConvArgs a{};
@@ -358,7 +361,7 @@ int slamhip_causal_conv_fwd(const void* x, const long long* strides, const float
 }
 
 size_t slamhip_causal_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
-  if (B <= 0 || C <= 0 || T < 0 || K < 2) return 0;
+  if (B <= 0 || C <= 0 || T < 0 || K < 2 || K > 4 || !conv_fits(B, T, C)) return 0;
   return (size_t)B * bwd_shape(B, T, C).gy * (K + 1) * C * sizeof(float);
 }
 
@@ -368,7 +371,7 @@ int slamhip_causal_conv_bwd(const void* dy, const void* x, const long long* stri
                             size_t workspace_bytes, void* stream) {
   SLAMHIP_REQUIRE(B >= 0 && T >= 0 && C > 0 && K >= 2 && K <= 4 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG,
                   "causal_conv_bwd: need C >= 1, 2 <= K <= 4 and a known type");
-  SLAMHIP_REQUIRE(B <= 65535 && T <= (1 << 20) && C <= (1 << 20), SLAMHIP_E_SIZE, "causal_conv_bwd: at most 65535 sequences, 2^20 steps and channels");
+  SLAMHIP_REQUIRE(conv_fits(B, T, C), SLAMHIP_E_SIZE, "causal_conv_bwd: at most 65535 sequences, 2^20 steps and channels");
   SLAMHIP_REQUIRE(weight && dweight && (B == 0 || workspace) && (B == 0 || T == 0 || (dy && x && dx && strides)), SLAMHIP_E_ARG,
                   "causal_conv_bwd: null pointer");
   SLAMHIP_REQUIRE(workspace_bytes >= slamhip_causal_conv_bwd_workspace_bytes(B, T, C, K), SLAMHIP_E_ARG, "causal_conv_bwd: workspace too small");

@@ -25,6 +25,9 @@ constexpr unsigned scale_load(int row, int kb, int rows, int KB) {
   return row < rows && kb < KB ? ((unsigned)row * (unsigned)KB + (unsigned)kb) * 4u : kBeyond;
 }
 
+// both operands below 2 GB with the rows that tiles have behind the last; a larger product is refused and needs no workspace
+constexpr bool gemm_fits(int M, int N, int K) { return (M + 256LL) * K < (1LL << 31) && (N + 256LL) * K < (1LL << 31); }
+
 // The kernel by the number of rows and tiles, and parts of k where that leaves most CUs idle.
 struct GemmPlan {
   enum Kind { kRows, k256, k128, k128KW, k64x128KW, k64KW } kind;

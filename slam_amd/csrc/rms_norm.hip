@@ -399,7 +399,7 @@ int slamhip_rms_norm_fwd(const void* x, const void* residual, const float* weigh
 }
 
 size_t slamhip_rms_norm_bwd_workspace_bytes(long long rows, int C) {
-  if (rows <= 0 || C <= 0) return 0;
+  if (rows <= 0 || C <= 0 || C > kMaxNormC || rows > kMaxGroups) return 0;   // beyond the limits the call is refused
   const int parts = norm_parts(rows, C);
   return parts == 1 ? 0 : (size_t)parts * (size_t)C * sizeof(float);
 }

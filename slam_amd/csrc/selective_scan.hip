@@ -776,21 +776,26 @@ using namespace slamhip;
                             : (P) == 4 ? FN<float, 4>(__VA_ARGS__)   \
                                        : FN<float, 8>(__VA_ARGS__)))
 
+namespace {
+// the limits of the entry points; a size beyond them needs no workspace, because its call is refused
+bool scan_fits(int B, int T, int C) { return B <= 65535 && T <= (1 << 20) && C <= (1 << 20); }
+}  // namespace
+
 #define SLAMHIP_SCAN_SIZES(name)                                                                                               \
   SLAMHIP_REQUIRE(B >= 0 && T >= 0 && C > 0 && N > 0 && N <= 32 && (dtype == SLAMHIP_F32 || dtype == SLAMHIP_BF16), SLAMHIP_E_ARG, \
                   name ": need C >= 1, 1 <= N <= 32 and a known type");                                                        \
-  SLAMHIP_REQUIRE(B <= 65535 && T <= (1 << 20) && C <= (1 << 20), SLAMHIP_E_SIZE, name ": at most 65535 sequences, 2^20 steps and channels")
+  SLAMHIP_REQUIRE(scan_fits(B, T, C), SLAMHIP_E_SIZE, name ": at most 65535 sequences, 2^20 steps and channels")
 
 extern "C" {
 
 size_t slamhip_selective_scan_kept_floats(int B, int T, int C, int N) {
-  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32 || !scan_fits(B, T, C)) return 0;
   const int tb = kept_steps(scan_shape(B, T, C, N, false).P);
   return (size_t)B * ((T + tb - 1) / tb) * C * N;
 }
 
 size_t slamhip_selective_scan_fwd_workspace_bytes(int B, int T, int C, int N) {
-  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > 32 || !scan_fits(B, T, C)) return 0;
   const ScanShape g = scan_shape(B, T, C, N, false);
   if (g.chunks == 1) return 0;
   return ((size_t)B * (g.chunks + 1) * C * N + (size_t)B * g.chunks * C) * sizeof(float);
@@ -821,7 +826,7 @@ int slamhip_selective_scan_fwd(const void* u, const void* delta, const void* z, 
 }
 
 size_t slamhip_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N) {
-  if (B <= 0 || T < 0 || C <= 0 || N <= 0 || N > 32) return 0;
+  if (B <= 0 || T < 0 || C <= 0 || N <= 0 || N > 32 || !scan_fits(B, T, C)) return 0;
   const ScanShape g = scan_shape(B, T, C, N, true);
   const size_t carry = g.chunks > 1 ? (size_t)B * g.chunks * C * (N + 1) : 0;
   return (carry + (size_t)B * g.chunks * C * (N + 2) + (size_t)B * T * g.groups * 8 * g.P) * sizeof(float);

@@ -505,7 +505,7 @@ int slamhip_pad_cast_bf16(const float* src, void* dst, long long P, int C, int C
  * their gradients, statistics and recurrent states are float32.  Elements need their own alignment alone.  Outputs are fully
  * overwritten and overlap no input except where said.  Sums have a fixed order: identical inputs give identical bits.
  *
- * Root-mean-square norm of the rows of x [rows][C] (C <= 16384): s = x + residual, rounded to `dtype` (sum_out; residual and
+ * Root-mean-square norm of the rows of x [rows][C] (C <= 16384, rows < 2^24): s = x + residual, rounded to `dtype` (sum_out; residual and
  * sum_out may be NULL: s = x), rstd = (mean(s^2) + eps)^(-1/2), y = s rstd weight.  Outputs, each may be NULL but one:
  * sum_out, y, and y8 uint8 [rows][C] (e4m3) with scales float32 [rows][ceil(C/128)]: scale = max(max|y| / 448, 2^-100) over
  * 128 consecutive values of the unrounded y, y8 = the nearest of y / scale.  rstd float32 [rows] (may be NULL) is kept for the
@@ -535,7 +535,8 @@ int slamhip_gemm_nt_fp8(const void* a, const float* a_scales, const void* b, con
 
 /* Sequences are [B][T][C] with unit stride over C and any stride, in elements, of a sequence and of a step: `strides` (host
  * memory) holds {sequence, step} of each in the order named.  lengths int32 [B] (NULL: all T; values are clamped to 0..T): rows
- * at and behind a sequence's length are never used, whatever they hold, and are zero in y and in the gradients.
+ * at and behind a sequence's length are never used, whatever they hold, and are zero in y and in the gradients.  The state of a sequence
+ * of length 0 passes through and takes no part in anything else.  At most 65535 sequences, 2^20 steps and 2^20 channels.
  *
  * Short causal convolution over time with a filter for each channel, weight [C][K], 2 <= K <= 4: pre = bias + sum_k w[c][k]
  * xp[t + k], y = pre (silu == 0) or pre / (1 + e^-pre), where xp is the K - 1 rows of state_in [B][K-1][C] (NULL: zeros) and
@@ -556,7 +557,8 @@ int slamhip_causal_conv_bwd(const void* dy, const void* x, const long long* stri
  * delta_bias itself with softplus == 0), h_t[c][n] = exp(dt A[c][n]) h_{t-1}[c][n] + dt u Bm[n], y = (sum_n Cm[n] h_t[c][n] +
  * D[c] u) z / (1 + e^-z).  D, delta_bias, z may be NULL (no such term; no gate).  state_in [B][C][N] (NULL: zeros) is h before
  * the first step, state_out [B][C][N] (NULL, or state_in itself) h after the sequence's last step; one frame at a time is T = 1.
- * kept_states: slamhip_selective_scan_kept_floats floats for the backward pass, or NULL.
+ * kept_states: slamhip_selective_scan_kept_floats floats for the backward pass, or NULL.  exp(A sum dt) over any stretch of a
+ * sequence has to be a float32 (states may grow, with A dt positive, that far).
  * strides: u, delta, z, Bm, Cm, y (z's may be anything without z). */
 size_t slamhip_selective_scan_kept_floats(int B, int T, int C, int N);
 size_t slamhip_selective_scan_fwd_workspace_bytes(int B, int T, int C, int N);

@@ -5,7 +5,8 @@
 //
 // A thread walks a few channels down a run of time steps with the last K rows in registers, so a row is read from memory
 // once but for the K - 1 rows in front of a run (and, backward, as many behind it).  Bytes bound this: 8 x 2048 x 4096 bfloat16 takes
-// 55 us forward (268 MB, 4.9 TB/s) and 97 us back (403 MB, 4.2 TB/s), 32 x 1 x 4096 with its states 5 us: a launch and two ways to memory.
+// 55 us forward (268 MB, 4.9 TB/s) and 99-106 us back (403 MB, 3.8-4.1 TB/s), in float32 101 and 183 us (5.3 and 4.4 TB/s); 32 x 1 x 4096
+// with its states 5 us: a launch and two ways to memory.
 #include <hip/hip_runtime.h>
 
 #include "common.h"

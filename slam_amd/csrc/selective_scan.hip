@@ -12,7 +12,9 @@
 // 64 channels.  Vector instructions bound it: an exponential (two issue slots), two products and two multiply-adds for every (step, channel,
 // state), and once a step and channel softplus, gate, sums over the quad.  At 8 x 2048 x 2048 x 16 bfloat16 the passes of 99 and 180 us
 // forward issue 23 and 34 vector instructions a step of a wave (16 and 20 of them the recurrence) and keep the units busy 81 and 84 % of
-// the time; those of 108 and 495 us back 24 and 101, 83 %.  The bytes alone would take 153 us.
+// the time; those of 108 and 495 us back 24 and 101, 83 %.  The bytes alone would take 153 us; float32 takes as long.  With 17 to 32 states the
+// pass back needs 379 registers, which leaves one wave a SIMD, and keeps 68 bytes of them in memory: 8 x 2048 x 1024 x 32 takes 86 + 146 us
+// forward and 91 + 577 us back.
 // A long sequence is cut into chunks where there are too few channels to fill the chip: a first pass leaves each chunk's own end
 // state and its sum of dt (the decay over a chunk is exp(A sum dt)), and every chunk of the second pass joins those in front of
 // it.  The backward pass runs over the chunks the same way from behind, and recomputes the states of TB steps from the one that

@@ -9,9 +9,13 @@ there is no autograd: a backward pass is a call of its own.  The checks are nati
 ValueError (what the tensors show) or RuntimeError (the library's limits of sizes and
 combinations) and launches nothing.  Outputs share no memory with each other or with
 inputs where a call does not say so.  Activations are float32 or bfloat16, parameters,
-statistics and states float32.  Workspaces are torch allocations of the call.
+statistics and states float32.  Workspaces are torch allocations of the call.  Limits:
+sequences B <= 65535, T and C <= 2^20; norms of fewer than 2^24 rows; operands of the
+product below 2 GB.  In a padded batch a sequence of length 0 may have anything in its
+state: it passes through and takes no part in the parameters' gradients.
 """
 import ctypes
+import sys
 
 import torch
 
@@ -21,7 +25,8 @@ from .encoder_ops import BF16, F32  # noqa: F401  (the activations' types)
 try:
     from .._lib import _sequence
 except ImportError as e:
-    raise RuntimeError("slam_amd: _lib/_sequence.so cannot be loaded (%s) - build it with `make -C slam_amd/csrc`; there is no fallback" % e)
+    raise RuntimeError("slam_amd: _lib/_sequence.so cannot be loaded (%s) - build it with `make -C slam_amd/csrc binding PYTHON=%s`; there is no fallback"
+                       % (e, sys.executable))
 
 FP8 = torch.float8_e4m3fn
 
@@ -56,7 +61,7 @@ def quantize_fp8_blocks(x, q, scales):
 def gemm_nt_fp8(a8, a_scales, b8, b_scales, out):
     """out [M, N] (bfloat16) = a8 . b8^T of e4m3 operands a8 [M, K], b8 [N, K], where each 128 values of an a8 row have
     a scale, a_scales [M, ceil(K / 128)], and each 128 x 128 block of b8 one, b_scales [ceil(N / 128), ceil(K / 128)]: what
-    quantize_fp8 (or rms_norm_fwd) and quantize_fp8_blocks write.  K a multiple of 16."""
+    quantize_fp8 (or rms_norm_fwd) and quantize_fp8_blocks write.  K a multiple of 16, a8 and b8 16-byte aligned."""
     _sequence.gemm_nt_fp8(a8, a_scales, b8, b_scales, out)
 
 
@@ -88,8 +93,8 @@ def selective_scan_fwd(u, delta, A, Bm, Cm, y, D=None, z=None, delta_bias=None, 
     takes delta + delta_bias as it is.  state_in [B, C, N] (None: zeros) is h before the first step and state_out h after the last,
     to be state_in of the call that continues the sequences (one frame at a time: T = 1); it may be state_in itself.  lengths
     (int32 [B], taken into [0, T]) bounds each sequence: rows behind it are not used and are zero in y.  kept_states (selective_scan_kept_states)
-    is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T.  States grow where A is positive:
-    exp(A sum dt) over up to a few hundred steps has to be a float32."""
+    is what selective_scan_bwd needs.  Sequences may be views with any strides over B and T.  States grow where A dt is
+    positive (positive A; with softplus=False negative steps too): exp(A sum dt) over any stretch of a sequence has to be a float32."""
     _sequence.selective_scan_fwd(u, delta, A, Bm, Cm, y, D, z, delta_bias, softplus, state_in, state_out, kept_states, lengths)
 
 

@@ -320,7 +320,7 @@ int slamhip_gemm_nt_fp8(const void* a, const float* a_scales, const void* b, con
                         void* workspace, size_t workspace_bytes, void* stream) {
   SLAMHIP_REQUIRE(M >= 0 && N >= 0 && K > 0, SLAMHIP_E_ARG, "gemm_nt_fp8: need M, N >= 0 and K >= 1");
   SLAMHIP_REQUIRE(K % 16 == 0, SLAMHIP_E_SIZE, "gemm_nt_fp8: K must be a multiple of 16");
-  SLAMHIP_REQUIRE(gemm_fits(M, N, K), SLAMHIP_E_SIZE, "gemm_nt_fp8: an operand is larger than 2 GB");
+  SLAMHIP_REQUIRE(gemm_fits(M, N, K), SLAMHIP_E_SIZE, "gemm_nt_fp8: an operand with 256 rows more is larger than 2 GB");
   if (M == 0 || N == 0) return SLAMHIP_OK;
   SLAMHIP_REQUIRE(a && a_scales && b && b_scales && out, SLAMHIP_E_ARG, "gemm_nt_fp8: null pointer");
   SLAMHIP_REQUIRE(((uintptr_t)a & 15) == 0 && ((uintptr_t)b & 15) == 0, SLAMHIP_E_ARG, "gemm_nt_fp8: operands must be 16-byte aligned");

@@ -11,7 +11,7 @@ combinations) and launches nothing.  Outputs share no memory with each other or 
 inputs where a call does not say so.  Activations are float32 or bfloat16, parameters,
 statistics and states float32.  Workspaces are torch allocations of the call.  Limits:
 sequences B <= 65535, T and C <= 2^20; norms of fewer than 2^24 rows; operands of the
-product below 2 GB.  In a padded batch a sequence of length 0 may have anything in its
+product with (rows + 256) K < 2^31.  In a padded batch a sequence of length 0 may have anything in its
 state: it passes through and takes no part in the parameters' gradients.
 """
 import ctypes
